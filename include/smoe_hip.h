@@ -236,8 +236,10 @@ int smoe_hip_set_stream(SmoeMetalCtx* ctx, void* hip_stream);
 
 /* Synchronise the context's stream and report the device-side error flags
  * raised since the last call, then clear them: a timed-out routing exchange
- * inside smoe_hip_moe_decode / smoe_hip_moe_decode_stack (SMOE_ERR_HIP) or an
- * expert id >= n_experts given to smoe_hip_permute (SMOE_ERR_ARG).  After a
+ * inside smoe_hip_moe_decode / smoe_hip_moe_decode_stack (SMOE_ERR_HIP), an
+ * expert id >= n_experts given to smoe_hip_permute (SMOE_ERR_ARG), or a row
+ * offset, slot, position or length outside its buffer given to the attention
+ * of prompts and of the 4-bit cache (SMOE_ERR_ARG).  After a
  * time-out every decode result since the previous call is suspect (waves of
  * the failed launch may have published words tagged for later launches), so
  * the call also clears the context's decode exchange words (epochs included)
@@ -422,6 +424,129 @@ int smoe_hip_matvec_group_bf16(SmoeMetalCtx* ctx, const uint16_t* const* w, cons
  * grows outside graph capture (else SMOE_ERR_CAPTURE). */
 int smoe_hip_attention_layer(SmoeMetalCtx* ctx, const SmoeAttnLayerArgs* args);
 
+/* ---- attention of prompts and over a 4-bit cache ---------------------------
+ * The single-token layer above for many rows at once: rows of many tokens or
+ * sequences, on device pointers, asynchronous on the context stream.  Common
+ * rules of this section:
+ *   - type: the element type of a call's rows (SMOE_TYPE_*).  Sums, softmax
+ *     and norms are fp32 (16-bit types: the softmax weights are rounded to the
+ *     type before they meet V); results are rounded once;
+ *   - rows lie a stride (elements) apart, heads side by side in a row.  Rows
+ *     are 16-byte aligned and their strides multiples of 16 bytes, up to 2^22
+ *     elements, so q, k and v may be column ranges of one matrix;
+ *   - head_dim 64, 128 or 256; num_heads a multiple of num_kv_heads (query
+ *     head i uses KV head i / (num_heads / num_kv_heads)), up to 1024;
+ *   - packed sequences: sequence b has rows offsets[b] .. offsets[b+1]-1;
+ *     offsets ascend, and rows outside every sequence are neither read nor
+ *     written;
+ *   - offsets, slots, positions and lengths live on the device.  One that
+ *     points outside its buffer is never followed: the call skips or zeroes
+ *     what it concerns and the next smoe_hip_synchronize returns SMOE_ERR_ARG;
+ *   - scratch (parts of split keys) grows outside graph capture; under capture
+ *     a call needs that of an earlier call of the same sizes, else
+ *     SMOE_ERR_CAPTURE.  The calls of a context share it: calls, and replays
+ *     of graphs captured from it, that may run at the same time need contexts
+ *     of their own. */
+#define SMOE_TYPE_F32   0
+#define SMOE_TYPE_F16   1
+#define SMOE_TYPE_BF16  2
+
+/* RMSNorm of every head (x / sqrt(mean(x^2) + 1e-6) * w, decode.cpp:155-167) and
+ * RoPE of its pairs (d, d + head_dim/2) by row positions[row] of the tables
+ * (decode.cpp:168-186), for n_rows rows of q [n_rows x num_heads x head_dim] and
+ * k [n_rows x num_kv_heads x head_dim].  The outputs may be the inputs (same
+ * pointer and stride).  q and q_out, or k and k_out, may be NULL: no such rows.
+ * q_norm_w / k_norm_w [head_dim] bf16, NULL: no norm.  rope_cos / rope_sin
+ * [n_positions x head_dim/2], both NULL: no rotation. */
+typedef struct {
+    const void*     q;
+    void*           q_out;
+    const void*     k;
+    void*           k_out;
+    const uint16_t* q_norm_w;
+    const uint16_t* k_norm_w;
+    const float*    rope_cos;
+    const float*    rope_sin;
+    const int32_t*  positions;      /* [n_rows] */
+    uint64_t q_stride, q_out_stride, k_stride, k_out_stride;
+    uint32_t n_rows, n_positions, num_heads, num_kv_heads, head_dim, type;
+} SmoeQkRowsArgs;
+int smoe_hip_qk_norm_rope(SmoeMetalCtx* ctx, const SmoeQkRowsArgs* args);
+
+/* Causal attention of whole prompts: query i of a sequence with n_q queries and
+ * n_k keys sees its keys 0 .. i + n_k - n_q (its last keys are its queries' own,
+ * so a prompt can be taken in chunks); a query that sees no key gets zeros.
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j
+ * q / out [q_rows x num_heads x head_dim], k / v [k_rows x num_kv_heads x
+ * head_dim]; k_offsets NULL: q_offsets.  max_k: keys of the longest sequence as
+ * far as known, 0: k_rows; it only decides how the work is split.  out must not
+ * overlap the inputs.  The weight of a key that a query does not see is exactly
+ * 0, so v has to be finite wherever another query of the sequence sees it. */
+typedef struct {
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    void*          out;
+    const int32_t* q_offsets;       /* [n_seqs + 1] */
+    const int32_t* k_offsets;       /* [n_seqs + 1] or NULL */
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+    uint32_t n_seqs, q_rows, k_rows, max_k;
+    uint32_t num_heads, num_kv_heads, head_dim, type;
+    float    scale;                 /* > 0 */
+} SmoePromptAttnArgs;
+int smoe_hip_attention_prompt(SmoeMetalCtx* ctx, const SmoePromptAttnArgs* args);
+
+/* A KV cache in 4 bits, buffers of the caller's: n_slots sequences of up to
+ * `capacity` positions.  Codes [n_slots][num_kv_heads][capacity][head_dim/2], two
+ * a byte (low nibble = even dim), and for each group of 64 dims a bf16 scale and
+ * min, [n_slots][num_kv_heads][capacity][head_dim/64][2]: value = code * scale +
+ * min, the SMOE_QUANT_Q4_SCALE_MIN format and quantizer (above).  144 bytes a
+ * position and KV head for head_dim 128 (K and V together), 1024 in fp32.
+ * Buffers 16-byte aligned. */
+typedef struct {
+    uint8_t*  k_codes;
+    uint8_t*  v_codes;
+    uint16_t* k_params;
+    uint16_t* v_params;
+    uint32_t  n_slots, capacity, num_kv_heads, head_dim;
+} SmoeKv4Cache;
+
+/* K and V rows [n_rows x num_kv_heads x head_dim] of packed sequences and where
+ * they lie in a cache: row offsets[b] + i at position start[b] + i of slot
+ * slots[b].  offsets NULL: one row a sequence (n_rows = n_seqs); slots NULL:
+ * sequence b in slot b. */
+typedef struct {
+    void*          k;
+    void*          v;
+    const int32_t* offsets;         /* [n_seqs + 1] or NULL */
+    const int32_t* slots;           /* [n_seqs] or NULL */
+    const int32_t* start;           /* [n_seqs] */
+    int32_t*       lens_out;        /* append: [n_seqs] start + rows, or NULL; not start itself */
+    uint64_t k_stride, v_stride;
+    uint32_t n_seqs, n_rows, type;
+} SmoeKv4RowsArgs;
+/* rows -> cache (finite values).  Where sequences of one call name the same place,
+ * the last one's row is kept; rows whose place is outside the cache are dropped. */
+int smoe_hip_kv4_append(SmoeMetalCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4RowsArgs* rows);
+/* cache -> rows; a place outside the cache reads as zeros (lens_out must be NULL) */
+int smoe_hip_kv4_read(SmoeMetalCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4RowsArgs* rows);
+
+/* Attention of one token a sequence (GQA, decode.cpp:190-227) over the first
+ * lens[b] positions of slot slots[b]: out [n_seqs x num_heads x head_dim] from q
+ * of the same shape; lens[b] = 0 gives zeros.  max_len: the longest length as far
+ * as known, 0: capacity; it only decides how the work is split (a captured graph
+ * follows lens). */
+typedef struct {
+    const void*    q;
+    void*          out;
+    const int32_t* slots;           /* [n_seqs] or NULL */
+    const int32_t* lens;            /* [n_seqs] */
+    uint64_t q_stride, out_stride;
+    uint32_t n_seqs, max_len, num_heads, type;
+    float    scale;                 /* > 0 */
+} SmoeKv4AttnArgs;
+int smoe_hip_attention_kv4(SmoeMetalCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* args);
+
 /* ---- .smoe vault -> HBM-resident expert pool ---------------------------
  * Replaces the reference's expert streamer for this path
  * (src/io/streamer.cpp parse_vault:183-212, main.cpp read_vault_header:96-157,
@@ -494,8 +619,8 @@ int smoe_hip_moe_decode_static(const SmoeMoeShape* shape, const SmoeMoeLayer* la
  * When enabled, every kernel the context launches outside graph capture is
  * bracketed by HIP events on the stream it runs on; profile_read returns the
  * launch count and summed event time of one kernel kind.  A kind that takes two
- * dispatches a call (PERMUTE over several segments, ATTENTION over several
- * context splits) counts one launch with the time of both. */
+ * dispatches a call (PERMUTE over several segments, the ATTENTION kinds over
+ * several parts of the keys) counts one launch with the time of both. */
 #define SMOE_KERNEL_MOE_UP        0   /* RMSNorm + router + top-k + gate/up GEMV + SiLU */
 #define SMOE_KERNEL_GATE_UP       1   /* gate/up GEMV + SiLU (reference surface)        */
 #define SMOE_KERNEL_MOE_DOWN      2   /* down GEMV + weighted combine + residual        */
@@ -512,7 +637,11 @@ int smoe_hip_moe_decode_static(const SmoeMoeShape* shape, const SmoeMoeLayer* la
 #define SMOE_KERNEL_ATTENTION    14   /* dense trunk: QK norm/RoPE/KV append + decode attention   */
 #define SMOE_KERNEL_STREAM       15   /* measurement: streaming-read ceiling (smoe_hip_stream_read) */
 #define SMOE_KERNEL_CHAIN        17 /* decode: every layer in one launch, the one-launch layer's schedule per layer */
-#define SMOE_KERNEL_KINDS        20
+#define SMOE_KERNEL_QK_ROWS      18   /* QK norm + RoPE of rows                                   */
+#define SMOE_KERNEL_ATTENTION_PROMPT 19 /* causal attention of packed prompts (and its join)      */
+#define SMOE_KERNEL_KV4_ROWS     20   /* rows into the 4-bit cache, and back                       */
+#define SMOE_KERNEL_ATTENTION_KV4 21  /* attention over the 4-bit cache (and its join)            */
+#define SMOE_KERNEL_KINDS        22
 int smoe_hip_profile_enable(SmoeMetalCtx* ctx, int enable);
 int smoe_hip_profile_read(SmoeMetalCtx* ctx, uint32_t kernel, uint64_t* launches, double* total_ms);
 

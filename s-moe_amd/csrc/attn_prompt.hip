@@ -1,0 +1,410 @@
+// attn_prompt.hip -- causal attention of whole prompts (gfx950):
+//
+//   o_i = sum_{j <= i + n_k - n_q} p_ij v_j / sum_j p_ij,  p_ij = 2^(s_ij - max_j s_ij),
+//   s_ij = scale log2(e) q_i . k_j
+//
+// over packed sequences (n_q query rows, n_k >= n_q key rows or fewer) with `group`
+// query heads on each KV head.
+//
+//   k_attn_prompt   one block per (row tile, KV head, part of the keys), four waves.
+//     Rows.  A tile's rows are (query, head of the group) pairs, the head fastest: all
+//     rows of a tile read the same K and V whatever the group, and with a group of 8
+//     a tile of 128 rows spans 16 queries, so little of the causal diagonal is wasted
+//     and a call of few tokens still fills its tiles.
+//     Products.  Both run transposed, S^T = K Q^T and O^T = V^T P^T, on 32x32 MFMA:
+//     a lane then holds the scores of ONE row (column l & 31), so maximum, sum, mask
+//     and rescaling are per-lane values, and the scores' registers are the next
+//     product's B operand as they stand (lane half h has keys 8b + 4h + i; V^T is
+//     read in that key order).  The rows' only exchange is between lanes l and l ^ 32.
+//     Tiles.  K and V tiles go to LDS by direct loads, one tile ahead, in 16-byte
+//     pieces whose place in a row is exchanged (kswz, vswz) so that the operand reads
+//     meet no bank twice: K as 16-byte pieces of 32 rows, V (16 bits) by transposing
+//     reads of 8 rows, V (32 bits) as dwords.
+//     f32 runs on v_mfma_f32_32x32x2_f32 throughout, 16-bit types on
+//     v_mfma_f32_32x32x16 with P rounded to their type (their sums are of the
+//     unrounded P, in fp32).
+//   k_prompt_join   where the keys were split: the parts of each row rescaled to
+//     their common maximum and normalised.
+#include <algorithm>
+
+#include "attn_common.hpp"
+#include "kernels.hpp"
+
+namespace smoe {
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_THREADS = PA_WAVES * WAVE;
+constexpr int PA_ROWS = PA_WAVES * 32;          // rows of a tile
+
+template <int HD, typename T>
+struct PromptShape {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int KT = F32 || HD == 256 ? 32 : 64;      // keys of a tile
+    static constexpr int RB = HD * static_cast<int>(sizeof(T));  // bytes of a K or V row
+    static constexpr int CPR = RB / 16;                          // 16-byte pieces of a row
+    static constexpr int TILE = KT * RB;                         // bytes of a K or V tile
+    static constexpr int LDS = 4 * TILE;                         // two tiles each of K and V
+    static constexpr int PER_WAVE = 2 * TILE / 1024 / PA_WAVES;  // direct loads a wave and tile
+    static constexpr int WAVES_PER_SIMD = HD == 256 ? 1 : 2;
+    // piece c of row r stands at piece c ^ kswz(r) (K), c ^ vswz(r) (V): the rows that one
+    // pass of an operand read touches then lie in different banks of the 256-byte width
+    __host__ __device__ static constexpr int kswz(int r) { return RB >= 256 ? (r & 15) : ((r >> 1) & 7); }
+    __host__ __device__ static constexpr int vswz(int r)
+    {
+        return F32 ? ((r >> 2) & 1) << 3 : RB >= 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+    }
+};
+
+// lane l's 16 bytes at base + off (off per lane) land at LDS byte address lds + 16 l
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+
+// The sequence and row tile of block tile `tile`, by the whole wave; false past the last one.
+__device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, uint32_t& seq, uint32_t& local)
+{
+    uint32_t base = 0;
+    for (uint32_t i = 0; i < p.n_seqs; i += WAVE) {
+        const uint32_t b = i + lane;
+        uint32_t n = 0;
+        if (b < p.n_seqs) {
+            const int32_t a = p.q_offsets[b], z = p.q_offsets[b + 1];
+            if (a >= 0 && z >= a && static_cast<uint32_t>(z) <= p.q_rows)
+                n = (static_cast<uint32_t>(z - a) * p.group + PA_ROWS - 1) / PA_ROWS;
+            else if (tile == 0)
+                flag_range(p.err);
+        }
+        uint32_t upto = n;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const uint32_t t = __shfl_up(upto, o);
+            if (lane >= o) upto += t;
+        }
+        const uint64_t past = __ballot(base + upto > tile);
+        if (past) {
+            const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            seq = i + f;
+            local = tile - base - (readlane_u32(upto, f) - readlane_u32(n, f));
+            return true;
+        }
+        base += readlane_u32(upto, WAVE - 1);
+    }
+    return false;
+}
+
+template <int HD, typename T>
+__global__ __launch_bounds__(PA_THREADS, (PromptShape<HD, T>::WAVES_PER_SIMD))
+void k_attn_prompt(PromptAttn p)
+{
+    using S = PromptShape<HD, T>;
+    constexpr int KT = S::KT, RB = S::RB, NSUB = KT / 32, ND = HD / 32;
+    extern __shared__ __align__(16) uint8_t smem[];
+
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
+
+    // ---- the block's tile, KV head and part ----------------------------------
+    // Consecutive blocks go to the eight XCDs in turn: where the KV heads divide them
+    // (or they divide the heads), a head's blocks stay on its XCDs and share their L2.
+    const uint32_t nkv = p.num_kv_heads;
+    uint32_t kvh, tile;
+    if (8 % nkv == 0) {
+        const uint32_t per = 8 / nkv, x = blockIdx.x & 7;
+        kvh = x / per;
+        tile = (blockIdx.x >> 3) * per + x % per;
+    } else if (nkv % 8 == 0) {
+        const uint32_t per = nkv / 8, r = blockIdx.x >> 3;
+        kvh = (blockIdx.x & 7) * per + r % per;
+        tile = r / per;
+    } else {
+        kvh = blockIdx.x % nkv;
+        tile = blockIdx.x / nkv;
+    }
+    uint32_t seq, local;
+    if (!find_tile(p, tile, lane, seq, local)) return;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    local = __builtin_amdgcn_readfirstlane(local);
+    const int32_t q0 = p.q_offsets[seq], nq = p.q_offsets[seq + 1] - q0;
+    const int32_t k0 = p.k_offsets[seq], k1 = p.k_offsets[seq + 1];
+    if (k0 < 0 || k1 < k0 || static_cast<uint32_t>(k1) > p.k_rows) {
+        if (threadIdx.x == 0) flag_range(p.err);
+        return;
+    }
+    const int32_t nk = k1 - k0, before = nk - nq;               // query i sees keys 0 .. i + before
+    const uint32_t G = p.group, rows = static_cast<uint32_t>(nq) * G;
+    // the longest tiles of a sequence first: what is left for the end of the launch is short
+    const uint32_t tiles = (rows + PA_ROWS - 1) / PA_ROWS;
+    const uint32_t r0 = (tiles - 1 - local) * PA_ROWS;
+    const uint32_t r = r0 + wv * 32 + col;
+    const bool live = r < rows;
+    const uint32_t qi = min(r, rows - 1) / G, g = min(r, rows - 1) % G;
+    const int32_t limit = live ? static_cast<int32_t>(qi) + before : -1;     // the row's last key
+    // last key of the block, first and last key limits of the wave's rows
+    const int32_t blk_last = static_cast<int32_t>((min(r0 + PA_ROWS, rows) - 1) / G) + before;
+    const uint32_t w0 = min(r0 + wv * 32, rows - 1), w1 = min(r0 + wv * 32 + 31, rows - 1);
+    const bool wave_full = r0 + wv * 32 + 31 < rows;
+    const int32_t wave_first = wave_full ? static_cast<int32_t>(w0 / G) + before : -1;
+    const int32_t wave_last = r0 + wv * 32 < rows ? static_cast<int32_t>(w1 / G) + before : -1;
+
+    int32_t t0 = 0, t1 = blk_last < 0 ? 0 : blk_last / KT + 1;
+    if (p.splits > 1) {
+        const int32_t part = (t1 + static_cast<int32_t>(p.splits) - 1) / static_cast<int32_t>(p.splits);
+        t0 = min(t1, static_cast<int32_t>(blockIdx.y) * part);
+        t1 = min(t1, t0 + part);
+    }
+
+    // ---- the wave's query rows: B operands --------------------------------------
+    const uint32_t head = kvh * G + g;
+    const T* qrow = static_cast<const T*>(p.q) + (static_cast<size_t>(q0) + qi) * p.q_stride + head * HD;
+    constexpr int QN = HD / (S::F32 ? 8 : 16);
+    uint4 qf[QN];
+#pragma unroll
+    for (int s = 0; s < QN; ++s) qf[s] = load_u4(reinterpret_cast<const uint8_t*>(qrow) + 32 * s + 16 * h);
+
+    // ---- direct loads: K and V tile t into buffer b ----------------------------
+    const uint64_t kb = p.k_stride * sizeof(T), vb = p.v_stride * sizeof(T);
+    const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + static_cast<uint64_t>(k0) * kb + kvh * RB;
+    const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + static_cast<uint64_t>(k0) * vb + kvh * RB;
+    const uint32_t lds0 = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem));
+    auto issue = [&](int32_t t, int b) {
+        const uint8_t* kt = kbase + static_cast<uint64_t>(t) * KT * kb;
+        const uint8_t* vt = vbase + static_cast<uint64_t>(t) * KT * vb;
+        const int32_t last = nk - 1 - t * KT;                   // keys past the end: the last one again (masked)
+        constexpr int N = S::PER_WAVE / 2;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int at = (wv * N + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
+            const uint32_t src = static_cast<uint32_t>(min(row, last));
+            load_to_lds(kt, src * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row)),
+                        lds0 + b * 2 * S::TILE + (wv * N + u) * 1024);
+            load_to_lds(vt, src * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row)),
+                        lds0 + b * 2 * S::TILE + S::TILE + (wv * N + u) * 1024);
+        }
+    };
+
+    f32x16_t acc[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    float mx = -INFINITY, sum = 0.f;
+    const float c2 = p.scale_log2;
+
+    auto tile_step = [&](int32_t t, int b) {
+        const uint8_t* kl = smem + b * 2 * S::TILE;
+        const uint8_t* vl = kl + S::TILE;
+        // ---- S^T = K Q^T ----
+        f32x16_t s[NSUB];
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < QN; ++ks) {
+                const uint4 a = *reinterpret_cast<const uint4*>(kl + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col)));
+                if constexpr (S::F32) {
+                    const f32x4v_t af = __builtin_bit_cast(f32x4v_t, a), bf = __builtin_bit_cast(f32x4v_t, qf[ks]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], s[u], 0, 0, 0);
+                } else if constexpr (__is_same(T, _Float16)) {
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                                  __builtin_bit_cast(f16x8_t, qf[ks]), s[u], 0, 0, 0);
+                } else {
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                                   __builtin_bit_cast(bf16x8_t, qf[ks]), s[u], 0, 0, 0);
+                }
+            }
+        }
+        // ---- the causal mask: keys t KT + 32 u + 8 (i / 4) + 4 h + i % 4 ----
+        if (t * KT + KT - 1 > wave_first) {
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int32_t key = t * KT + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
+                    if (key > limit) s[u][i] = -INFINITY;
+                }
+        }
+        // ---- running maximum and sum ----
+        float mt = s[0][0];
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[u][i]);
+        mt = half_max(mt);
+        if (__ballot(mt > mx)) {
+            const float mn = fmaxf(mx, mt);
+            const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f((mx - mn) * c2) : 0.f;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            mx = mn;
+        }
+        const float mc = mx > -INFINITY ? mx * c2 : 0.f;        // (no key yet: every weight 0)
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c2, -mc));
+                sum += s[u][i];
+            }
+        // ---- O^T += V^T P^T ----
+        if constexpr (S::F32) {
+#pragma unroll
+            for (int kk = 0; kk < KT / 8; ++kk)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const int c = 8 * d + col / 4;
+                        const float a = *reinterpret_cast<const float*>(vl + (8 * kk + 4 * h + j) * RB +
+                                                                        16 * (c ^ (h << 3)) + 4 * (col & 3));
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kk / 4][(kk % 4) * 4 + j], acc[d], 0, 0, 0);
+                    }
+        } else {
+            // lane (16-lane group g4 = 2 h + ..., place c) of a transposing read names row c / 4
+            // and dims 4 (c % 4) .. of 16; it receives the rows' values of dim c
+            const int c = lane & 15, vrow = 4 * h + (c >> 2);
+#pragma unroll
+            for (int ks = 0; ks < KT / 16; ++ks) {
+                uint4 pb;
+                const f32x16_t& sv = s[ks / 2];
+                const int o = (ks % 2) * 8;
+                pb.x = pack2<T>(sv[o + 0], sv[o + 1]);
+                pb.y = pack2<T>(sv[o + 2], sv[o + 3]);
+                pb.z = pack2<T>(sv[o + 4], sv[o + 5]);
+                pb.w = pack2<T>(sv[o + 6], sv[o + 7]);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint8_t* a = vl + (16 * ks + vrow) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
+                                       32 * ((lane >> 4) & 1) + 8 * (c & 3);
+                    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+                    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
+                    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 8 * RB));
+                    typedef short s16x8_t __attribute__((ext_vector_type(8)));
+                    const s16x8_t av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (__is_same(T, _Float16))
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, av),
+                                                                        __builtin_bit_cast(f16x8_t, pb), acc[d], 0, 0, 0);
+                    else
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av),
+                                                                         __builtin_bit_cast(bf16x8_t, pb), acc[d], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    if (t0 < t1) issue(t0, 0);
+    for (int32_t t = t0; t < t1; ++t) {
+        const int b = (t - t0) & 1;
+        // this wave's part of tile t has arrived and its reads of the other buffer are done; after
+        // the barrier so are every wave's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 1 < t1) issue(t + 1, b ^ 1);
+        if (t * KT <= wave_last) tile_step(t, b);
+    }
+
+    // ---- the result -----------------------------------------------------------
+    sum = half_sum(sum);
+    if (!live) return;
+    const size_t row_out = static_cast<size_t>(q0) + qi;
+    if (p.splits == 1) {
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        T* out = static_cast<T*>(p.out) + row_out * p.out_stride + head * HD;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = acc[d][4 * i] * inv, x1 = acc[d][4 * i + 1] * inv, x2 = acc[d][4 * i + 2] * inv,
+                            x3 = acc[d][4 * i + 3] * inv;
+                T* o = out + 32 * d + 8 * i + 4 * h;
+                if constexpr (S::F32) *reinterpret_cast<float4*>(o) = make_float4(x0, x1, x2, x3);
+                else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
+            }
+    } else {
+        const size_t nrow = static_cast<size_t>(p.q_rows) * nkv * G;
+        const size_t at = (row_out * nkv * G + head) * p.splits + blockIdx.y;
+        if (h == 0) {
+            p.part[2 * at] = mx > -INFINITY ? mx * c2 : -INFINITY;
+            p.part[2 * at + 1] = sum;
+        }
+        if (sum == 0.f) return;                                  // (the join reads no such part)
+        float* out = p.part + part_acc_at(nrow, p.splits) + at * HD;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(out + 32 * d + 8 * i + 4 * h) =
+                    make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+    }
+}
+
+// one wave per (query row, head) of the sequences
+template <int HD, typename T>
+__global__ __launch_bounds__(PA_THREADS)
+void k_prompt_join(PromptAttn p)
+{
+    const int lane = threadIdx.x & 63;
+    const uint32_t heads = p.num_kv_heads * p.group;
+    const uint32_t w = blockIdx.x * PA_WAVES + (threadIdx.x >> 6), row = w / heads;
+    if (row >= p.q_rows || static_cast<int32_t>(row) < p.q_offsets[0] ||
+        static_cast<int32_t>(row) >= p.q_offsets[p.n_seqs])
+        return;
+    const size_t nrow = static_cast<size_t>(p.q_rows) * heads, at = static_cast<size_t>(w) * p.splits;
+    float o[HD / WAVE];
+    join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(nrow, p.splits) + at * HD, p.splits, lane, o);
+    store_row<HD>(static_cast<T*>(p.out) + row * p.out_stride + (w % heads) * HD, o, lane);
+}
+
+void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k)
+{
+    a.tiles = static_cast<uint32_t>(static_cast<uint64_t>(a.q_rows) * a.group / PA_ROWS) + a.n_seqs;
+    const uint32_t kt = type == SMOE_TYPE_F32 || head_dim == 256 ? 32 : 64;
+    // full tiles alone: a part-filled one of each sequence may not exist
+    const uint64_t blocks = std::max<uint64_t>(
+        1, (static_cast<uint64_t>(a.q_rows) * a.group + PA_ROWS - 1) / PA_ROWS * a.num_kv_heads);
+    const uint32_t want = static_cast<uint32_t>(std::min<uint64_t>(JOIN_MAX, 512 / blocks));
+    // a part has four tiles or more
+    a.splits = std::max<uint32_t>(1, std::min<uint32_t>(want, max_k / (4 * kt)));
+}
+
+size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t head_dim)
+{
+    if (a.splits == 1) return 0;
+    return part_floats(static_cast<size_t>(a.q_rows) * a.num_kv_heads * a.group, a.splits, head_dim) * sizeof(float);
+}
+
+hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t head_dim, uint32_t type, hipStream_t s)
+{
+    return with_type_and_head(type, head_dim, [&](auto t, auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        using T = decltype(t);
+        constexpr uint32_t lds = PromptShape<HD, T>::LDS;
+        static_assert(lds <= 160 * 1024, "LDS of a CU");
+        if constexpr (lds > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_prompt<HD, T>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e != hipSuccess) return e;
+        }
+        // every XCD has as many blocks of a tile row where KV heads share or split XCDs
+        const uint32_t nkv = a.num_kv_heads;
+        const uint32_t per = 8 % nkv == 0 ? 8 / nkv : 1;
+        const uint32_t blocks = (a.tiles + per - 1) / per * per * nkv;
+        launch_kernel_lds(k_attn_prompt<HD, T>, dim3(blocks, a.splits), dim3(PA_THREADS), lds, s, a);
+        if (a.splits > 1) {
+            const uint32_t waves = a.q_rows * nkv * a.group;
+            launch_kernel(k_prompt_join<HD, T>, dim3((waves + PA_WAVES - 1) / PA_WAVES), dim3(PA_THREADS), s, a);
+        }
+        return hipGetLastError();
+    });
+}
+
+}  // namespace smoe

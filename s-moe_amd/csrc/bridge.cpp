@@ -15,6 +15,7 @@
 #include <cstring>
 #include <vector>
 
+#include "context.hpp"
 #include "kernels.hpp"
 #include "shape.hpp"
 
@@ -146,6 +147,8 @@ struct SmoeMetalCtx {
     float* mv_in = nullptr;          // reference-surface GEMV staging
     uint8_t* attn_part = nullptr;    // decode attention: per-(head, split) partials + counters
     size_t attn_part_cap = 0;        // bytes
+    Buf<float> attn_rows;            // prompt and 4-bit-cache attention: parts of split keys
+    std::vector<float*> attn_rows_old;   // outgrown, but captured graphs may hold them
     float* mv_out = nullptr;
     uint32_t mv_cap = 0;
     uint64_t perm_cap = 0;
@@ -491,6 +494,52 @@ void* dispatch_group(SmoeMetalCtx* ctx, const smoe::ExpertTable& tbl, uint32_t n
 }  // namespace
 
 // ============================================================================
+// what attention.cpp uses of a context (context.hpp)
+// ============================================================================
+namespace smoe {
+
+ContextView context_view(const SmoeMetalCtx* ctx) { return {ctx->device, ctx->stream, ctx->d_err}; }
+
+int context_attention_scratch(SmoeMetalCtx* ctx, size_t bytes, float** p)
+{
+    Buf<float>& b = ctx->attn_rows;
+    const size_t n = (bytes + sizeof(float) - 1) / sizeof(float);
+    const bool capturing = stream_capturing(ctx->stream);
+    if (b.n < n) {
+        if (capturing) return context_refuse(ctx, SMOE_ERR_CAPTURE, "the attention scratch would grow under capture");
+        // (twice what a captured graph keeps alive, so that what stays behind is bounded)
+        const size_t want = b.captured ? std::max(n, 2 * b.n) : n;
+        float* grown = nullptr;
+        if (!dalloc(ctx, &grown, want)) return SMOE_ERR_HIP;
+        if (b.p && b.captured) {
+            ctx->attn_rows_old.push_back(b.p);
+        } else if (b.p) {
+            // hipFree waits for the device, so for earlier calls that use it too
+            dfree(b.p);
+        }
+        b = Buf<float>{};
+        b.p = grown;
+        b.n = want;
+    }
+    b.captured |= capturing;
+    *p = b.p;
+    return SMOE_OK;
+}
+
+int context_launch(SmoeMetalCtx* ctx, uint32_t kind, const char* what, hipError_t (*launch)(void*), void* arg)
+{
+    return timed(ctx, kind, what, [&] { return launch(arg); }) ? SMOE_OK : SMOE_ERR_HIP;
+}
+
+int context_refuse(SmoeMetalCtx* ctx, int rc, const char* why)
+{
+    std::snprintf(ctx->last_err, sizeof(ctx->last_err), "%s", why);
+    return rc;
+}
+
+}  // namespace smoe
+
+// ============================================================================
 // 1. reference surface
 // ============================================================================
 extern "C" SmoeMetalCtx* smoe_metal_init(size_t slot_bytes)
@@ -545,6 +594,8 @@ extern "C" void smoe_metal_destroy(SmoeMetalCtx* ctx)
     dfree(ctx->mv_in);
     dfree(ctx->mv_out);
     dfree(ctx->attn_part);
+    dfree(ctx->attn_rows.p);
+    for (float* p : ctx->attn_rows_old) dfree(p);
     dfree(ctx->d_err);
     dfree(ctx->d_input);
     dfree(ctx->d_hidden);
@@ -867,7 +918,8 @@ extern "C" int smoe_hip_synchronize(SmoeMetalCtx* ctx)
             std::snprintf(ctx->last_err, sizeof(ctx->last_err), "device:%s%s%s (flags %u)",
                           (e & 1u) ? " routing exchange timed out" : "", (e & 2u) ? " expert id out of range" : "",
                           (e & 4u) ? " a stack block ran off its XCD (later calls write exchange words through)"
-                                   : "",
+                          : (e & 8u) ? " attention: a row offset, slot, position or length out of range"
+                                     : "",
                           e);
             return (e & 5u) ? SMOE_ERR_HIP : SMOE_ERR_ARG;
         }

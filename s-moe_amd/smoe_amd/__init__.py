@@ -79,6 +79,45 @@ class SmoeAttnLayerArgs(C.Structure):
                 + [("attn_scale", C.c_float)])
 
 
+# element types of the rows of the prompt and 4-bit-cache attention calls
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+
+
+class SmoeQkRowsArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "q_out", "k", "k_out", "q_norm_w", "k_norm_w", "rope_cos",
+                                           "rope_sin", "positions")]
+                + [(n, C.c_uint64) for n in ("q_stride", "q_out_stride", "k_stride", "k_out_stride")]
+                + [(n, C.c_uint32) for n in ("n_rows", "n_positions", "num_heads", "num_kv_heads", "head_dim",
+                                             "type")])
+
+
+class SmoePromptAttnArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "q_offsets", "k_offsets")]
+                + [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+                + [(n, C.c_uint32) for n in ("n_seqs", "q_rows", "k_rows", "max_k", "num_heads", "num_kv_heads",
+                                             "head_dim", "type")]
+                + [("scale", C.c_float)])
+
+
+class SmoeKv4Cache(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k_codes", "v_codes", "k_params", "v_params")]
+                + [(n, C.c_uint32) for n in ("n_slots", "capacity", "num_kv_heads", "head_dim")])
+
+
+class SmoeKv4RowsArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "offsets", "slots", "start", "lens_out")]
+                + [(n, C.c_uint64) for n in ("k_stride", "v_stride")]
+                + [(n, C.c_uint32) for n in ("n_seqs", "n_rows", "type")])
+
+
+class SmoeKv4AttnArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "out", "slots", "lens")]
+                + [(n, C.c_uint64) for n in ("q_stride", "out_stride")]
+                + [(n, C.c_uint32) for n in ("n_seqs", "max_len", "num_heads", "type")]
+                + [("scale", C.c_float)])
+
+
 class SmoeExpertBlob(C.Structure):
     _fields_ = [("packed_gate", C.c_void_p), ("scales_gate", C.c_void_p),
                 ("packed_up", C.c_void_p), ("scales_up", C.c_void_p),
@@ -124,6 +163,11 @@ SIGNATURES = [
     ("smoe_hip_matvec_group_bf16", _I, [_VP, C.POINTER(_VP), C.POINTER(_VP), C.POINTER(_VP),
                                         C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), _U32]),
     ("smoe_hip_attention_layer", _I, [_VP, C.POINTER(SmoeAttnLayerArgs)]),
+    ("smoe_hip_qk_norm_rope", _I, [_VP, C.POINTER(SmoeQkRowsArgs)]),
+    ("smoe_hip_attention_prompt", _I, [_VP, C.POINTER(SmoePromptAttnArgs)]),
+    ("smoe_hip_kv4_append", _I, [_VP, C.POINTER(SmoeKv4Cache), C.POINTER(SmoeKv4RowsArgs)]),
+    ("smoe_hip_kv4_read", _I, [_VP, C.POINTER(SmoeKv4Cache), C.POINTER(SmoeKv4RowsArgs)]),
+    ("smoe_hip_attention_kv4", _I, [_VP, C.POINTER(SmoeKv4Cache), C.POINTER(SmoeKv4AttnArgs)]),
     ("smoe_hip_vault_open", _I, [C.c_char_p, C.POINTER(_VP)]),
     ("smoe_hip_vault_close", None, [_VP]),
     ("smoe_hip_vault_info", _I, [_VP, C.POINTER(SmoeVaultInfo)]),
@@ -143,11 +187,13 @@ KERNEL_MOE_UP, KERNEL_GATE_UP, KERNEL_MOE_DOWN, KERNEL_DOWN_SLOTS, KERNEL_TOPK =
 KERNEL_PERMUTE, KERNEL_GROUPED_GATE_UP, KERNEL_GROUPED_DOWN, KERNEL_SCATTER = 5, 6, 7, 8
 KERNEL_ROUTE, KERNEL_SPLIT, KERNEL_MOE_LAYER = 9, 10, 12
 KERNEL_GEMV, KERNEL_ATTENTION, KERNEL_STREAM, KERNEL_CHAIN = 13, 14, 15, 17
+KERNEL_QK_ROWS, KERNEL_ATTENTION_PROMPT, KERNEL_KV4_ROWS, KERNEL_ATTENTION_KV4 = 18, 19, 20, 21
 DECODE_LAUNCHES, DECODE_SPLIT, DECODE_CHAIN = 0, 2, 4
 KERNEL_NAMES = {0: "moe_up", 1: "gate_up", 2: "moe_down", 3: "down_slots", 4: "topk",
                 5: "permute", 6: "grouped_gate_up", 7: "grouped_down", 8: "combine", 9: "route",
                 10: "split", 12: "moe_layer", 13: "gemv", 14: "attention",
-                15: "stream_read", 17: "moe_chain"}
+                15: "stream_read", 17: "moe_chain", 18: "qk_rows", 19: "attention_prompt",
+                20: "kv4_rows", 21: "attention_kv4"}
 
 _lib = None
 
@@ -268,6 +314,21 @@ class Context:
             self.lib.smoe_metal_attention_layer(self.ptr, C.byref(args))
         else:
             self._check(self.lib.smoe_hip_attention_layer(self.ptr, C.byref(args)), "attention_layer")
+
+    def qk_norm_rope(self, args: "SmoeQkRowsArgs"):
+        self._check(self.lib.smoe_hip_qk_norm_rope(self.ptr, C.byref(args)), "qk_norm_rope")
+
+    def attention_prompt(self, args: "SmoePromptAttnArgs"):
+        self._check(self.lib.smoe_hip_attention_prompt(self.ptr, C.byref(args)), "attention_prompt")
+
+    def kv4_append(self, cache: "SmoeKv4Cache", rows: "SmoeKv4RowsArgs"):
+        self._check(self.lib.smoe_hip_kv4_append(self.ptr, C.byref(cache), C.byref(rows)), "kv4_append")
+
+    def kv4_read(self, cache: "SmoeKv4Cache", rows: "SmoeKv4RowsArgs"):
+        self._check(self.lib.smoe_hip_kv4_read(self.ptr, C.byref(cache), C.byref(rows)), "kv4_read")
+
+    def attention_kv4(self, cache: "SmoeKv4Cache", args: "SmoeKv4AttnArgs"):
+        self._check(self.lib.smoe_hip_attention_kv4(self.ptr, C.byref(cache), C.byref(args)), "attention_kv4")
 
     def set_decode_engine(self, engine: int):
         """DECODE_CHAIN (one launch per step, the default), DECODE_LAUNCHES (per-layer
