@@ -502,7 +502,7 @@ int smoe_hip_attention_prompt(SmoeMetalCtx* ctx, const SmoePromptAttnArgs* args)
  * min, [n_slots][num_kv_heads][capacity][head_dim/64][2]: value = code * scale +
  * min, the SMOE_QUANT_Q4_SCALE_MIN format and quantizer (above).  144 bytes a
  * position and KV head for head_dim 128 (K and V together), 1024 in fp32.
- * Buffers 16-byte aligned. */
+ * Buffers 16-byte aligned, capacity up to 2^24. */
 typedef struct {
     uint8_t*  k_codes;
     uint8_t*  v_codes;

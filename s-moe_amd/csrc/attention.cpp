@@ -12,6 +12,7 @@ namespace {
 constexpr uint64_t kMostRows = 1ull << 31;      // rows times heads of a call
 constexpr uint64_t kMostStride = 1ull << 22;    // elements between rows
 constexpr uint32_t kMostHeads = 1024;
+constexpr uint32_t kMostPositions = 1u << 24;   // of a cache slot
 
 bool bad_type(uint32_t t) { return t != SMOE_TYPE_F32 && t != SMOE_TYPE_F16 && t != SMOE_TYPE_BF16; }
 bool bad_head_dim(uint32_t d) { return d != 64 && d != 128 && d != 256; }
@@ -77,8 +78,9 @@ int check_cache(SmoeMetalCtx* ctx, const SmoeKv4Cache* c)
         return refuse(ctx, SMOE_ERR_ARG, "a NULL or empty cache");
     if (bad_head_dim(c->head_dim)) return refuse(ctx, SMOE_ERR_SHAPE, "head_dim is not 64, 128 or 256");
     if (c->num_kv_heads > kMostHeads) return refuse(ctx, SMOE_ERR_SHAPE, "more than 1024 heads");
-    if (c->n_slots > 0x7FFFFFFFu || c->capacity > 0x7FFFFFE0u)
-        return refuse(ctx, SMOE_ERR_SHAPE, "slots or positions past 31 bits");
+    // (a slot's codes of one head are addressed in 32 bits)
+    if (c->n_slots > 0x7FFFFFFFu || c->capacity > kMostPositions)
+        return refuse(ctx, SMOE_ERR_SHAPE, "more than 2^31 slots or 2^24 positions");
     if (misaligned(c->k_codes, 16) || misaligned(c->v_codes, 16) || misaligned(c->k_params, 16) ||
         misaligned(c->v_params, 16))
         return refuse(ctx, SMOE_ERR_ARG, "a cache buffer is not 16-byte aligned");

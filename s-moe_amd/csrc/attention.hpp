@@ -92,6 +92,7 @@ struct Kv4Attn {
     uint32_t n_seqs, group;     // group: query heads per KV head
     float scale_log2;
     uint32_t splits;            // parts of a sequence's positions, joined by a second launch
+    uint32_t part_tiles;        // length of a part; more where a sequence would have more than `splits`
     float* part;                // rows = sequences times heads (part_floats)
     uint32_t* err;
 };

@@ -10,15 +10,21 @@
 //     (two codes a word by one and-or with the bits of 1024 or 64 and one packed
 //     subtraction), the scales and mins are applied to the fp32 sums of a group:
 //       q . k_j = sum_g s_g (sum c q) + m_g (sum_g q)
-//     The query is put in f16 twice, the value and what its rounding left (22 bits;
-//     a power of two a head keeps it in range), so a score is as exact as an fp32 sum.
+//     The query goes in as f16, at a power of two a head that keeps it in range: exact
+//     for 16-bit types; f32 twice, the value and what its rounding left (22 bits).
 //     Scores come out transposed, S^T = K Q^T: lane (m = l & 15, q = l >> 4) has the
 //     scores of head m at positions 4 q + i (+ 16), which are the B operand of the
 //     weighted sum O^T = V^T P^T as they stand.  P is multiplied by the V scale of its
-//     position and group first and put in f16 twice like q, at a power of two that the
-//     largest scale of the group so far sets: the mins' part, sum p m_g, is one fp32 sum a group.
-//     K rows are read 8 bytes a lane and group (16 dims), V rows 2 bytes (4 dims of
-//     group g: 64 g + 4 m), the next tile's while this one is computed.
+//     position and group first and put in f16 (bf16 results: once, its 11 bits against
+//     the result's 8; else twice like q), at a power of two that the largest scale of the
+//     group so far sets: the mins' part, sum p m_g, is one fp32 sum a group.
+//     A tile's bytes come by direct loads into the wave's own two LDS buffers, one tile
+//     ahead, with no register held meanwhile: 128 registers leave four waves a SIMD, whose
+//     loads in flight and whose arithmetic cover each other.  K operands are 8-byte reads
+//     (16 dims of a position), V operands 4-bit transposing reads (a lane gets 8 positions
+//     of two dims); 16-byte pieces of a row are exchanged so that neither meets a bank
+//     twice.  The 16 lanes that share a position would unpack the same scales and mins, so
+//     each pair is put into floats by one lane and passed on through LDS.
 //   k_kv4_join   the parts of each (sequence, head) joined.
 #include <algorithm>
 
@@ -32,12 +38,20 @@ constexpr int KA_THREADS = KA_WAVES * WAVE;
 constexpr int KA_TILE = 32;             // positions of a wave step
 constexpr int KA_HEADS = 16;            // query heads of a block (MFMA columns)
 
+// A constant that the compiler holds in a vector register: (w & mask) | bits is then one
+// v_and_or_b32, which takes no literals.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t c)
+{
+    uint32_t r;
+    asm("v_mov_b32 %0, %1" : "=v"(r) : "s"(c));
+    return r;
+}
 // 8 codes of a word as f16: codes 0 4 | 1 5 | 2 6 | 3 7
-__device__ __forceinline__ f16x8_t codes8(uint32_t w)
+__device__ __forceinline__ f16x8_t codes8(uint32_t w, uint32_t even, uint32_t odd)
 {
     const uint32_t v = w >> 8;
-    const uint4 b = make_uint4((w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x54005400u,
-                               (v & 0x000F000Fu) | 0x64006400u, (v & 0x00F000F0u) | 0x54005400u);
+    const uint4 b = make_uint4((w & even) | 0x64006400u, (w & odd) | 0x54005400u, (v & even) | 0x64006400u,
+                               (v & odd) | 0x54005400u);
     const _Float16 lo = static_cast<_Float16>(-1024.f), hi = static_cast<_Float16>(-64.f);
     const f16x8_t bias = {lo, lo, hi, hi, lo, lo, hi, hi};
     return __builtin_bit_cast(f16x8_t, b) + bias;
@@ -66,99 +80,163 @@ __device__ __forceinline__ float quads_sum(float v)
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return half_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
-__device__ __forceinline__ uint32_t quads_max_u32(uint32_t v)
+// maximum over the lanes that agree in l % N (N = 1, 2, 4), left in every lane
+template <int N>
+__device__ __forceinline__ uint32_t residue_max(uint32_t v)
 {
+    if constexpr (N < 2) v = max(v, dpp_u32<DPP_QUAD_XOR1>(0u, v));
+    if constexpr (N < 4) v = max(v, dpp_u32<DPP_QUAD_XOR2>(0u, v));
+    v = max(v, dpp_u32<DPP_ROW_ROR4>(0u, v));
+    v = max(v, dpp_u32<DPP_ROW_ROR8>(0u, v));
     const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = max(a[0], a[1]);
     const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(b[0], b[1]);
 }
+// orders this wave's LDS writes before its later reads of other lanes' values, and reads before writes
+__device__ __forceinline__ void wave_lds_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// lane l's 16 (4) bytes at base + off (off per lane) land at LDS byte address lds + 16 l (4 l)
+__device__ __forceinline__ void lds_load16(const void* base, uint32_t off, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void lds_load4(const void* base, uint32_t off, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
 
-// the raw bytes of 32 positions that a lane needs
-template <int NG>
-struct Kv4Tile {
-    uint2 k[2][NG];          // codes of position 16 u + m, dims 64 g + 16 q ..
-    uint32_t v[8][NG];       // codes of position 16 (j / 4) + 4 q + j % 4, dims 64 g + 4 m ..
-    uint32_t kp[8][NG];      // scale | min << 16 of the same positions
-    uint32_t vp[8][NG];
+// a wave's buffer of one tile: K codes, V codes (rows of RB bytes), then the scale and min
+// words of K and of V as they are, later the floats of one of them
+template <int HD>
+struct Kv4Shape {
+    static constexpr int NG = HD / 64;
+    static constexpr int RB = HD / 2, PIECES = RB / 16;
+    static constexpr int CODES = KA_TILE * RB;
+    static constexpr int NC = CODES / 1024;                    // direct loads of a tile's codes
+    static constexpr int PAIRS = KA_TILE * NG;
+    static constexpr int NP = (PAIRS + 63) / 64;               // direct loads of a tile's pairs
+    static constexpr int BUF = 2 * CODES + 2 * NP * 256;
+    static constexpr int RS = HD + 4;                          // padded row of a head in the merge
+    static constexpr int LDS = KA_WAVES * (2 * BUF > KA_HEADS * RS * 4 ? 2 * BUF : KA_HEADS * RS * 4);
+    static constexpr int WAVES_PER_SIMD = HD == 256 ? 2 : 4;
+    static_assert(2 * PAIRS * 4 <= 2 * NP * 256, "the floats of K or V fit the words' place");
+    // piece c of row r stands at piece c ^ swz(r)
+    __host__ __device__ static constexpr int swz(int r) { return r / (256 / RB) & (PIECES - 1); }
 };
 
 template <int HD, typename T>
-__global__ __launch_bounds__(KA_THREADS, (HD == 256 ? 1 : 2))
+__global__ __launch_bounds__(KA_THREADS, (Kv4Shape<HD>::WAVES_PER_SIMD))
 void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 {
-    constexpr int NG = HD / 64;
-    constexpr int RS = HD + 4;                  // padded row of a head in LDS
-    extern __shared__ __align__(16) float buf[];    // [KA_WAVES][KA_HEADS][RS]
+    using S = Kv4Shape<HD>;
+    constexpr int NG = S::NG, RB = S::RB, RS = S::RS;
+    constexpr bool Q2 = sizeof(T) == 4;         // q as two f16
+    constexpr bool P2 = !__is_same(T, __bf16);  // P as two f16
+    extern __shared__ __align__(16) float buf[];    // the waves' tiles; before and after, rows of heads
     __shared__ float qsum[KA_HEADS * NG], mw[KA_WAVES * KA_HEADS], lw[KA_WAVES * KA_HEADS];
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m16 = lane & 15, q = lane >> 4;
     const uint32_t G = p.group, nkv = p.c.num_kv_heads;
-    const uint32_t sub = blockIdx.x % n_sub, kvh = blockIdx.x / n_sub % nkv, seq = blockIdx.x / n_sub / nkv;
+    const uint32_t sub = blockIdx.x % n_sub, kvh = blockIdx.x / n_sub % nkv;
+    // the sequences one further with every part: else those that share a remainder of the XCDs'
+    // number would all run on one XCD (32 of 52 to 8192 positions: 31 us against 26)
+    const uint32_t seq = (blockIdx.x / n_sub / nkv + blockIdx.y) % p.n_seqs;
     const uint32_t hbase = kvh * G + sub * KA_HEADS;            // first query head of the block
     const uint32_t ng = min(static_cast<uint32_t>(KA_HEADS), G - sub * KA_HEADS);
+    const uint32_t heads = nkv * G;
+    const size_t nrow = static_cast<size_t>(p.n_seqs) * heads;
 
     // ---- the block's positions ------------------------------------------------
-    const int32_t slot = p.slots ? p.slots[seq] : static_cast<int32_t>(seq), len = p.lens[seq];
+    const int32_t slot = __builtin_amdgcn_readfirstlane(p.slots ? p.slots[seq] : static_cast<int32_t>(seq));
+    const int32_t len = __builtin_amdgcn_readfirstlane(p.lens[seq]);
     uint32_t n = static_cast<uint32_t>(len);
     if (static_cast<uint32_t>(slot) >= p.c.n_slots || len < 0 || n > p.c.capacity) {
         if (threadIdx.x == 0) flag_range(p.err);
         n = 0;                                                  // (a row of zeros)
     }
-    const uint32_t tiles = (n + KA_TILE - 1) / KA_TILE, part = (tiles + p.splits - 1) / p.splits;
+    // parts of `part` tiles, so that sequences of different lengths give blocks of the same work
+    const uint32_t tiles = (n + KA_TILE - 1) / KA_TILE, part = max(p.part_tiles, (tiles + p.splits - 1) / p.splits);
     const uint32_t t0 = min(tiles, blockIdx.y * part), t1 = min(tiles, t0 + part);
+    if (t0 >= t1 && p.splits > 1) {
+        if (threadIdx.x < ng) {
+            const size_t at = (static_cast<size_t>(seq) * heads + hbase + threadIdx.x) * p.splits + blockIdx.y;
+            p.part[2 * at] = -INFINITY;
+            p.part[2 * at + 1] = 0.f;
+        }
+        return;
+    }
     const size_t line0 = (static_cast<size_t>(n ? slot : 0) * nkv + kvh) * p.c.capacity;
-    const uint8_t* kc = p.c.codes[0] + line0 * (HD / 2);
-    const uint8_t* vc = p.c.codes[1] + line0 * (HD / 2);
-    const uint32_t* kpar = reinterpret_cast<const uint32_t*>(p.c.params[0]) + line0 * NG;
-    const uint32_t* vpar = reinterpret_cast<const uint32_t*>(p.c.params[1]) + line0 * NG;
+    const uint8_t* kc = p.c.codes[0] + line0 * RB;
+    const uint8_t* vc = p.c.codes[1] + line0 * RB;
+    const uint8_t* kpar = reinterpret_cast<const uint8_t*>(p.c.params[0]) + line0 * (4 * NG);
+    const uint8_t* vpar = reinterpret_cast<const uint8_t*>(p.c.params[1]) + line0 * (4 * NG);
 
-    // positions past the end: the last one again (masked, and its V weights 0)
-    auto load_tile = [&](uint32_t t, Kv4Tile<NG>& x) {
-        const uint32_t b = t * KA_TILE, last = n - 1;
+    // ---- direct loads of tile t into buffer b of this wave --------------------------
+    uint8_t* mine = reinterpret_cast<uint8_t*>(buf) + wv * (2 * S::BUF);
+    const uint32_t lds = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
+    auto issue = [&](uint32_t t, int b) {
+        const uint64_t at = static_cast<uint64_t>(t) * KA_TILE;
+        const uint32_t last = n - 1 - t * KA_TILE;              // past the end: the last position again
+        const uint32_t to = lds + b * S::BUF;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const size_t at = min(b + 16 * u + m16, last);
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-                x.k[u][g] = *reinterpret_cast<const uint2*>(kc + at * (HD / 2) + 32 * g + 8 * q);
+        for (int i = 0; i < S::NC; ++i) {
+            const int byte = i * 1024 + lane * 16, row = byte / RB, piece = (byte % RB / 16) ^ S::swz(row);
+            const uint32_t off = min(static_cast<uint32_t>(row), last) * RB + piece * 16;
+            lds_load16(kc + at * RB, off, to + i * 1024);
+            lds_load16(vc + at * RB, off, to + S::CODES + i * 1024);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const size_t at = min(b + 16 * (j / 4) + 4 * q + j % 4, last);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                x.v[j][g] = *reinterpret_cast<const uint16_t*>(vc + at * (HD / 2) + 32 * g + 2 * m16);
-                x.kp[j][g] = kpar[at * NG + g];
-                x.vp[j][g] = vpar[at * NG + g];
-            }
+        for (int i = 0; i < S::NP; ++i) {
+            const uint32_t pr = (lane + 64 * i) % S::PAIRS;
+            const uint32_t off = (min(pr / NG, last) * NG + pr % NG) * 4;
+            lds_load4(kpar + at * (4 * NG), off, to + 2 * S::CODES + i * 256);
+            lds_load4(vpar + at * (4 * NG), off, to + 2 * S::CODES + (S::NP + i) * 256);
         }
     };
-    Kv4Tile<NG> ta;
-    if (t0 + wv < t1) load_tile(t0 + wv, ta);
 
-    // ---- the query heads: scaled, then f16 halves ---------------------------------
-    for (uint32_t g = wv; g < KA_HEADS; g += KA_WAVES) {
-        const T* src = static_cast<const T*>(p.q) + seq * p.q_stride + (hbase + min(g, ng - 1)) * HD;
-        float x[HD / WAVE], top = 0.f;
+    if (t0 + wv < t1) issue(t0 + wv, 0);
+
+    // ---- the query heads: a power of two each, then f16 --------------------------
+    // (through the waves' second buffers, which the first tile leaves alone)
+    constexpr int HPW = KA_HEADS / KA_WAVES;
+    static_assert(HPW * RS * 4 <= S::BUF, "a wave's heads fit its second buffer");
+    auto head_row = [&](uint32_t g) {
+        return reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(buf) + g / HPW * (2 * S::BUF) + S::BUF) + g % HPW * RS;
+    };
+    float x[HPW][NG];
 #pragma unroll
-        for (int j = 0; j < HD / WAVE; ++j) {
-            x[j] = g < ng ? static_cast<float>(src[j * WAVE + lane]) * p.scale_log2 : 0.f;
-            top = fmaxf(top, fabsf(x[j]));
-        }
-        // a power of two that brings the largest value to 8 .. 16 (none for 0 or an infinity)
+    for (int i = 0; i < HPW; ++i) {
+        const uint32_t g = wv * HPW + i;
+        const T* src = static_cast<const T*>(p.q) + seq * p.q_stride + (hbase + min(g, ng - 1)) * HD;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) x[i][j] = static_cast<float>(src[j * WAVE + lane]);
+    }
+#pragma unroll
+    for (int i = 0; i < HPW; ++i) {
+        const uint32_t g = wv * HPW + i;
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) top = fmaxf(top, fabsf(x[i][j]));
+        // brings the largest value to 8 .. 16 (nothing for 0 or an infinity)
         const uint32_t e = (__float_as_uint(wave_max(top)) >> 23) & 0xFFu;
-        const uint32_t es = e == 0 || e == 255 ? 127u : min(max(e, 4u), 250u);
+        const uint32_t es = e == 0 || e == 255 ? 130u : min(max(e, 4u), 250u);
         const float down = __uint_as_float((257u - es) << 23);       // 2^(130 - es)
 #pragma unroll
-        for (int j = 0; j < HD / WAVE; ++j) {
-            x[j] *= down;
-            buf[g * RS + j * WAVE + lane] = x[j];
-            const float gs = wave_sum(x[j]);                      // group j
+        for (int j = 0; j < NG; ++j) {
+            const float v = g < ng ? x[i][j] * down : 0.f;
+            head_row(g)[j * WAVE + lane] = v;
+            const float gs = wave_sum(v);                     // group j
             if (lane == 0) qsum[g * NG + j] = gs;
         }
-        if (lane == 0) mw[g] = __uint_as_float((es - 3u) << 23);   // 2^(es - 130), 1 / down
+        if (lane == 0) mw[g] = __uint_as_float((es - 3u) << 23);     // 2^(es - 130)
     }
     __syncthreads();
     f16x8_t qh[NG][2], ql[NG][2];
@@ -168,7 +246,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
         qs[g] = qsum[m16 * NG + g];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float* r = buf + m16 * RS + 64 * g + 16 * q + 8 * i;
+            const float* r = head_row(m16) + 64 * g + 16 * q + 8 * i;
             uint4 hi, lo;
             split2(r[code_at(0)], r[code_at(1)], hi.x, lo.x);
             split2(r[code_at(2)], r[code_at(3)], hi.y, lo.y);
@@ -178,66 +256,101 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
             ql[g][i] = __builtin_bit_cast(f16x8_t, lo);
         }
     }
-    const float up = mw[m16];
+    const float up = mw[m16] * p.scale_log2;    // of the sums below: scores in powers of two
     __syncthreads();
 
     // ---- the positions --------------------------------------------------------------
+    const uint32_t even = in_vgpr(0x000F000Fu), odd = in_vgpr(0x00F000F0u);
     float mx = -INFINITY, sum = 0.f, vmin[NG];  // of head m16 (sums: this lane's positions)
-    f32x4v_t acc[NG][4];                        // dim 64 g + 4 (4 q + i) + d of head m16 at [g][d][i]
+    f32x4v_t acc[NG][4];                        // dim 64 g + 16 d + 4 q + i of head m16 at [g][d][i]
+    int ebits[NG];                              // exponent field of the group's largest V scale so far
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         vmin[g] = 0.f;
+        ebits[g] = 27;
 #pragma unroll
         for (int d = 0; d < 4; ++d) acc[g][d] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
     }
-    int ebits[NG];                              // exponent field of the group's largest V scale so far
-    float vup[NG];                              // 2^(14 - (ebits - 127)): brings P times a V scale under 2^15
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        ebits[g] = 27;
-        vup[g] = __builtin_amdgcn_ldexpf(1.f, 127 + 14 - 27);
-    }
 
-    auto step = [&](uint32_t t, const Kv4Tile<NG>& x) {
-        const uint32_t b = t * KA_TILE;
-        f32x4v_t sc[2];
+    // this lane's operand places in a buffer: K row 16 u + m16, V rows of positions 16 (k / 4) + 4 q + k % 4
+    // for k = m16 % 8 (dims 16 (2 e + m16 / 8) of a transposing read e)
+    const uint32_t kat = m16 * RB + (((q >> 1) ^ S::swz(m16)) * 16) + (q & 1) * 8;
+    const uint32_t vrow = 16 * ((m16 >> 2) & 1) + 4 * q + (m16 & 3);
+    const uint32_t vat = vrow * RB + (S::swz(vrow) * 16) + (m16 >> 3) * 8;
+    auto step = [&](uint32_t t, int b0) {
+        const uint8_t* kl = mine + b0 * S::BUF;
+        const uint8_t* vl = kl + S::CODES;
+        uint32_t* words = reinterpret_cast<uint32_t*>(mine + b0 * S::BUF + 2 * S::CODES);
+        float* par = reinterpret_cast<float*>(words);           // scale, min: [NG][KA_TILE] each
+        uint32_t kp[S::NP], vp[S::NP];
+#pragma unroll
+        for (int i = 0; i < S::NP; ++i) {
+            kp[i] = words[lane + 64 * i];
+            vp[i] = words[(S::NP + i) * 64 + lane];
+        }
+        // scales and mins as floats, one pair a lane; read back as the lane's positions 16 u + 4 q + 0 .. 3
+        auto put_pairs = [&](const uint32_t (&w)[S::NP], float f) {
+            wave_lds_order();
+#pragma unroll
+            for (int i = 0; i < S::NP; ++i) {
+                const uint32_t pr = (lane + 64 * i) % S::PAIRS, at = pr % NG * KA_TILE + pr / NG;
+                par[at] = __uint_as_float(w[i] << 16) * f;
+                par[NG * KA_TILE + at] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+            wave_lds_order();
+        };
+        auto pairs = [&](int what, int g, int u) {
+            return *reinterpret_cast<const f32x4v_t*>(par + (what * NG + g) * KA_TILE + 16 * u + 4 * q);
+        };
+        put_pairs(kp, 1.f);
+        // ---- scores ----
+        float s[8];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            sc[u] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
+            f32x4v_t sc;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 f32x4v_t d = {0.f, 0.f, 0.f, 0.f};
-                const f16x8_t c0 = codes8(x.k[u][g].x), c1 = codes8(x.k[u][g].y);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c0, ql[g][0], d, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c1, ql[g][1], d, 0, 0, 0);
+                const uint2 w = *reinterpret_cast<const uint2*>(kl + u * (16 * RB) + (kat ^ (32 * g)));
+                const f16x8_t c0 = codes8(w.x, even, odd), c1 = codes8(w.y, even, odd);
+                if constexpr (Q2) {
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c0, ql[g][0], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c1, ql[g][1], d, 0, 0, 0);
+                }
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c0, qh[g][0], d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(c1, qh[g][1], d, 0, 0, 0);
+                const f32x4v_t ks = pairs(0, g, u), km = pairs(1, g, u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w = x.kp[4 * u + i][g];
-                    sc[u][i] = fmaf(__uint_as_float(w << 16), d[i], fmaf(__uint_as_float(w & 0xFFFF0000u), qs[g], sc[u][i]));
-                }
+                for (int i = 0; i < 4; ++i)
+                    sc[i] = g ? fmaf(ks[i], d[i], fmaf(km[i], qs[g], sc[i])) : fmaf(ks[i], d[i], km[i] * qs[g]);
             }
-        }
-        float s[8], mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool in = b + 16 * (j / 4) + 4 * q + j % 4 < n;
-            s[j] = in ? sc[j / 4][j % 4] * up : -INFINITY;
-            mt = fmaxf(mt, s[j]);
+            for (int i = 0; i < 4; ++i) s[4 * u + i] = sc[i];
         }
+        const uint32_t b = t * KA_TILE;
+        if (b + KA_TILE > n) {
+            asm volatile("" : "+v"(s[0]));      // (a branch, not selects in every tile)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (b + 16 * (j / 4) + 4 * q + j % 4 >= n) s[j] = -INFINITY;
+        }
+        float mt = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int j = 2; j < 8; ++j) mt = fmaxf(mt, s[j]);
+        mt = quads_max(mt) * up;
         // V scales: the largest exponent of a group sets the power of two of its P
+        int eb[NG], e = 0;
         bool grown = false;
-        int eb[NG];
+        uint32_t vs = 0;
+#pragma unroll
+        for (int i = 0; i < S::NP; ++i) vs = max(vs, vp[i] & 0x7FFFu);
+        vs = residue_max<NG>(vs);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            uint32_t vs = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) vs = max(vs, x.vp[j][g] & 0x7FFFu);
-            eb[g] = static_cast<int>(__builtin_amdgcn_readfirstlane(quads_max_u32(vs)) >> 7);
-            grown |= eb[g] > ebits[g];
+            eb[g] = max(ebits[g], static_cast<int>(readlane_u32(vs, g) >> 7));
+            grown |= eb[g] != ebits[g];
+            e = lane % NG == g ? eb[g] : e;
         }
-        mt = quads_max(mt);
         if (__ballot(mt > mx) || grown) {
             const float mn = fmaxf(mx, mt);
             const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 0.f;
@@ -245,90 +358,86 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 vmin[g] *= f;
-                const int e = max(eb[g], ebits[g]);
-                const float fg = __builtin_amdgcn_ldexpf(f, ebits[g] - e);
-                ebits[g] = e;
-                vup[g] = __builtin_amdgcn_ldexpf(1.f, 127 + 14 - e);
+                const float fg = __builtin_amdgcn_ldexpf(f, ebits[g] - eb[g]);
+                ebits[g] = eb[g];
 #pragma unroll
                 for (int d = 0; d < 4; ++d) acc[g][d] *= fg;
             }
             mx = mn;
         }
+        put_pairs(vp, __builtin_amdgcn_ldexpf(1.f, 127 + 14 - e));     // P times a scale stays under 2^15
         const float m0 = mx > -INFINITY ? mx : 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            s[j] = __builtin_amdgcn_exp2f(s[j] - m0);
+            s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], up, -m0));
             sum += s[j];
         }
+        // ---- weighted values ----
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             uint4 hi, lo;
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t w = x.vp[j][g];
-                y[j] = s[j] * vup[g] * __uint_as_float(w << 16);
-                vmin[g] = fmaf(s[j], __uint_as_float(w & 0xFFFF0000u), vmin[g]);
+            for (int u = 0; u < 2; ++u) {
+                const f32x4v_t vs = pairs(0, g, u), vm = pairs(1, g, u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[4 * u + i] = s[4 * u + i] * vs[i];
+                    vmin[g] = fmaf(s[4 * u + i], vm[i], vmin[g]);
+                }
             }
-            split2(y[0], y[1], hi.x, lo.x);
-            split2(y[2], y[3], hi.y, lo.y);
-            split2(y[4], y[5], hi.z, lo.z);
-            split2(y[6], y[7], hi.w, lo.w);
+            // in the order of codes8's places
+            if constexpr (P2) {
+                split2(y[code_at(0)], y[code_at(1)], hi.x, lo.x);
+                split2(y[code_at(2)], y[code_at(3)], hi.y, lo.y);
+                split2(y[code_at(4)], y[code_at(5)], hi.z, lo.z);
+                split2(y[code_at(6)], y[code_at(7)], hi.w, lo.w);
+            } else {
+                hi = make_uint4(pack2<_Float16>(y[code_at(0)], y[code_at(1)]), pack2<_Float16>(y[code_at(2)], y[code_at(3)]),
+                                pack2<_Float16>(y[code_at(4)], y[code_at(5)]), pack2<_Float16>(y[code_at(6)], y[code_at(7)]));
+            }
             const f16x8_t ph = __builtin_bit_cast(f16x8_t, hi), pl = __builtin_bit_cast(f16x8_t, lo);
-            // positions j, j + 1 of a dim side by side
-            uint32_t w2[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w2[j] = x.v[2 * j][g] | (x.v[2 * j + 1][g] << 16);
+            for (int e2 = 0; e2 < 2; ++e2) {
+                typedef int i32x2_t __attribute__((ext_vector_type(2)));
+                typedef __attribute__((address_space(3))) i32x2_t lds_i32x2;
+                const i32x2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(vl + (vat ^ (32 * g + 16 * e2))));
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const uint32_t mask = d & 1 ? 0x00F000F0u : 0x000F000Fu, one = d & 1 ? 0x54005400u : 0x64006400u;
-                const _Float16 neg = static_cast<_Float16>(d & 1 ? -64.f : -1024.f);
-                const f16x8_t bias = {neg, neg, neg, neg, neg, neg, neg, neg};
-                const int sh = d & 2 ? 8 : 0;
-                const uint4 cb = make_uint4(((w2[0] >> sh) & mask) | one, ((w2[1] >> sh) & mask) | one,
-                                            ((w2[2] >> sh) & mask) | one, ((w2[3] >> sh) & mask) | one);
-                const f16x8_t cv = __builtin_bit_cast(f16x8_t, cb) + bias;
-                acc[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, pl, acc[g][d], 0, 0, 0);
-                acc[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, ph, acc[g][d], 0, 0, 0);
+                for (int d2 = 0; d2 < 2; ++d2) {
+                    const f16x8_t cv = codes8(static_cast<uint32_t>(w[d2]), even, odd);
+                    f32x4v_t& o = acc[g][2 * e2 + d2];
+                    if constexpr (P2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, pl, o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, ph, o, 0, 0, 0);
+                }
             }
         }
     };
-    if constexpr (HD <= 128) {
-        Kv4Tile<NG> tb;
-        for (uint32_t t = t0 + wv; t < t1; t += 2 * KA_WAVES) {
-            if (t + KA_WAVES < t1) load_tile(t + KA_WAVES, tb);
-            step(t, ta);
-            if (t + KA_WAVES >= t1) break;
-            if (t + 2 * KA_WAVES < t1) load_tile(t + 2 * KA_WAVES, ta);
-            step(t + KA_WAVES, tb);
-        }
-    } else {
-        // (no registers for a second tile)
-        for (uint32_t t = t0 + wv; t < t1; t += KA_WAVES) {
-            step(t, ta);
-            if (t + KA_WAVES < t1) load_tile(t + KA_WAVES, ta);
-        }
+    int b = 0;
+    for (uint32_t t = t0 + wv; t < t1; t += KA_WAVES, b ^= 1) {
+        // tile t has arrived, and nothing of the other buffer is still being read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (t + KA_WAVES < t1) issue(t + KA_WAVES, b ^ 1);
+        step(t, b);
     }
 
     // ---- merge: the four lanes of a head, then the waves, then parts ------------------
+    __syncthreads();                            // (every wave's tiles are read)
     sum = quads_sum(sum);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         vmin[g] = quads_sum(vmin[g]);
         const float down = __builtin_amdgcn_ldexpf(1.f, ebits[g] - 127 - 14);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)             // dims 64 g + 4 (4 q + i) + 0 .. 3
-            *reinterpret_cast<float4*>(buf + (wv * KA_HEADS + m16) * RS + 64 * g + 16 * q + 4 * i) =
-                make_float4(fmaf(acc[g][0][i], down, vmin[g]), fmaf(acc[g][1][i], down, vmin[g]),
-                            fmaf(acc[g][2][i], down, vmin[g]), fmaf(acc[g][3][i], down, vmin[g]));
+        for (int d = 0; d < 4; ++d)
+            *reinterpret_cast<float4*>(buf + (wv * KA_HEADS + m16) * RS + 64 * g + 16 * d + 4 * q) =
+                make_float4(fmaf(acc[g][d][0], down, vmin[g]), fmaf(acc[g][d][1], down, vmin[g]),
+                            fmaf(acc[g][d][2], down, vmin[g]), fmaf(acc[g][d][3], down, vmin[g]));
     }
     if (q == 0) {
         mw[wv * KA_HEADS + m16] = mx;
         lw[wv * KA_HEADS + m16] = sum;
     }
     __syncthreads();
-    const uint32_t heads = nkv * G;
-    const size_t nrow = static_cast<size_t>(p.n_seqs) * heads;
     for (uint32_t o = threadIdx.x; o < ng * HD; o += KA_THREADS) {
         const uint32_t g = o / HD, d = o % HD, head = hbase + g;
         float M = -INFINITY;
@@ -375,9 +484,13 @@ void kv4_plan(Kv4Attn& a, uint32_t head_dim, uint32_t max_len)
     const uint32_t n_sub = (a.group + KA_HEADS - 1) / KA_HEADS;
     const uint64_t blocks = static_cast<uint64_t>(a.n_seqs) * a.c.num_kv_heads * n_sub;
     const uint32_t tiles = max_len / KA_TILE + (max_len % KA_TILE != 0);
-    // some four blocks a CU, a tile a wave or more
-    const uint64_t want = std::min<uint64_t>(JOIN_MAX, std::max<uint64_t>(1, 1024 / std::max<uint64_t>(1, blocks)));
-    a.splits = std::max<uint32_t>(1, std::min<uint32_t>(static_cast<uint32_t>(want), tiles / KA_WAVES));
+    // As many blocks as are resident at once (256 CUs of four, or two at head_dim 256), each with a tile a
+    // wave or more: 16 sequences of 32768 over 4 KV heads 72.8 us in 16 parts (1024 blocks), 78.0 in 8, 74.8
+    // in 12, 76.2 in 24; one of 777 over 4 KV heads 6.9 us in 7 parts, 8.5 in 6, 15.5 in one.
+    const uint32_t resident = head_dim == 256 ? 512 : 1024;
+    const uint64_t most = std::min<uint64_t>(JOIN_MAX, resident / std::max<uint64_t>(1, blocks));
+    a.splits = std::max<uint32_t>(1, std::min<uint32_t>(static_cast<uint32_t>(most), (tiles + KA_WAVES - 1) / KA_WAVES));
+    a.part_tiles = (tiles + a.splits - 1) / a.splits;
 }
 
 size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t head_dim)
@@ -392,7 +505,7 @@ hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t head_dim, uint32_t ty
         constexpr int HD = decltype(hd)::value;
         using T = decltype(t);
         const uint32_t n_sub = (a.group + KA_HEADS - 1) / KA_HEADS, heads = a.c.num_kv_heads * a.group;
-        constexpr uint32_t lds = KA_WAVES * KA_HEADS * (HD + 4) * sizeof(float);
+        constexpr uint32_t lds = Kv4Shape<HD>::LDS;
         if constexpr (lds > 64 * 1024) {
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_kv4<HD, T>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);

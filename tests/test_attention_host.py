@@ -136,7 +136,7 @@ def test_prompt(lib, more, rc):
 
 CACHES = [(dict(k_codes=None), SMOE_ERR_ARG), (dict(v_params=None), SMOE_ERR_ARG), (dict(n_slots=0), SMOE_ERR_ARG),
           (dict(capacity=0), SMOE_ERR_ARG), (dict(num_kv_heads=0), SMOE_ERR_ARG), (dict(head_dim=80), SMOE_ERR_SHAPE),
-          (dict(v_codes=DEV + 8), SMOE_ERR_ARG), (dict(capacity=(1 << 31) - 1), SMOE_ERR_SHAPE),
+          (dict(v_codes=DEV + 8), SMOE_ERR_ARG), (dict(capacity=(1 << 24) + 1), SMOE_ERR_SHAPE),
           (dict(n_slots=1 << 31), SMOE_ERR_SHAPE)]
 
 
