@@ -72,6 +72,8 @@ struct PromptAttn {
     uint32_t n_seqs, q_rows, k_rows, num_kv_heads, group;
     float scale_log2;           // score scale times log2(e)
     uint32_t tiles;             // row tiles, at most (prompt_plan)
+    uint32_t row_waves;         // waves of 32 rows of a block's row tile
+    uint32_t key_groups;        // groups of such waves that take the tile's keys in turn
     uint32_t splits;            // parts of a sequence's keys, joined by a second launch
     float* part;                // rows = query rows times heads (part_floats)
     uint32_t* err;

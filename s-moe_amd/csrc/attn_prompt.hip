@@ -6,10 +6,11 @@
 // over packed sequences (n_q query rows, n_k >= n_q key rows or fewer) with `group`
 // query heads on each KV head.
 //
-//   k_attn_prompt   one block per (row tile, KV head, part of the keys), four waves.
+//   k_attn_prompt   one block per (row tile, KV head, part of the keys): RW waves of 32
+//     rows, KG groups of them that take the key tiles in turn and merge in LDS at the end.
 //     Rows.  A tile's rows are (query, head of the group) pairs, the head fastest: all
 //     rows of a tile read the same K and V whatever the group, and with a group of 8
-//     a tile of 128 rows spans 16 queries, so little of the causal diagonal is wasted
+//     a tile of 128 rows (RW = 4) spans 16 queries, so little of the causal diagonal is wasted
 //     and a call of few tokens still fills its tiles.
 //     Products.  Both run transposed, S^T = K Q^T and O^T = V^T P^T, on 32x32 MFMA:
 //     a lane then holds the scores of ONE row (column l & 31), so maximum, sum, mask
@@ -32,9 +33,7 @@
 
 namespace smoe {
 
-constexpr int PA_WAVES = 4;
-constexpr int PA_THREADS = PA_WAVES * WAVE;
-constexpr int PA_ROWS = PA_WAVES * 32;          // rows of a tile
+constexpr int JOIN_WAVES = 4;
 
 template <int HD, typename T>
 struct PromptShape {
@@ -44,7 +43,6 @@ struct PromptShape {
     static constexpr int CPR = RB / 16;                          // 16-byte pieces of a row
     static constexpr int TILE = KT * RB;                         // bytes of a K or V tile
     static constexpr int LDS = 4 * TILE;                         // two tiles each of K and V
-    static constexpr int PER_WAVE = 2 * TILE / 1024 / PA_WAVES;  // direct loads a wave and tile
     static constexpr int WAVES_PER_SIMD = HD == 256 ? 1 : 2;
     // piece c of row r stands at piece c ^ kswz(r) (K), c ^ vswz(r) (V): the rows that one
     // pass of an operand read touches then lie in different banks of the 256-byte width
@@ -62,47 +60,88 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint
                  : "memory", "m0");
 }
 
-// The sequence and row tile of block tile `tile`, by the whole wave; false past the last one.
-__device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, uint32_t& seq, uint32_t& local)
+template <typename T>
+__device__ __forceinline__ f32x16_t mma16(uint4 a, uint4 b, f32x16_t c)
+{
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+}
+// the two values of w added to c
+template <typename T>
+__device__ __forceinline__ float add2(uint32_t w, float c)
+{
+    if constexpr (__is_same(T, _Float16)) {
+        const f16x2_t one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), one, c, false);
+    } else {
+        const bf16x2_t one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), one, c, false);
+    }
+}
+
+// inclusive sum over the lanes up to this one
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
+{
+    v += dpp_u32<0x111>(0u, v);                 // row_shr 1, 2, 4, 8
+    v += dpp_u32<0x112>(0u, v);
+    v += dpp_u32<0x114>(0u, v);
+    v += dpp_u32<0x118>(0u, v);
+    v += dpp_u32<DPP_ROW_BCAST15, 0xA>(0u, v);
+    v += dpp_u32<DPP_ROW_BCAST31, 0xC>(0u, v);
+    return v;
+}
+
+// The sequence of row tile `tile` (ROWS rows each), by the whole wave; false past the last one.
+// Sequences whose offsets point outside their rows have no tiles.
+struct PromptSeq {
+    int32_t q0, nq, k0, nk;
+    uint32_t local;                             // tile of the sequence
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, PromptSeq& s)
 {
     uint32_t base = 0;
     for (uint32_t i = 0; i < p.n_seqs; i += WAVE) {
-        const uint32_t b = i + lane;
+        const uint32_t b = min(i + lane, p.n_seqs - 1);
+        const int32_t a = p.q_offsets[b], z = p.q_offsets[b + 1], ka = p.k_offsets[b], kz = p.k_offsets[b + 1];
+        const bool ok = a >= 0 && z >= a && static_cast<uint32_t>(z) <= p.q_rows && ka >= 0 && kz >= ka &&
+                        static_cast<uint32_t>(kz) <= p.k_rows;
         uint32_t n = 0;
-        if (b < p.n_seqs) {
-            const int32_t a = p.q_offsets[b], z = p.q_offsets[b + 1];
-            if (a >= 0 && z >= a && static_cast<uint32_t>(z) <= p.q_rows)
-                n = (static_cast<uint32_t>(z - a) * p.group + PA_ROWS - 1) / PA_ROWS;
-            else if (tile == 0)
-                flag_range(p.err);
+        if (i + lane < p.n_seqs) {
+            if (ok) n = (static_cast<uint32_t>(z - a) * p.group + ROWS - 1) / ROWS;
+            else if (tile == 0) flag_range(p.err);
         }
-        uint32_t upto = n;
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const uint32_t t = __shfl_up(upto, o);
-            if (lane >= o) upto += t;
-        }
-        const uint64_t past = __ballot(base + upto > tile);
+        const uint32_t upto = base + wave_scan(n);
+        const uint64_t past = __ballot(upto > tile);
         if (past) {
             const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            seq = i + f;
-            local = tile - base - (readlane_u32(upto, f) - readlane_u32(n, f));
+            s.q0 = __builtin_amdgcn_readlane(a, f);
+            s.nq = __builtin_amdgcn_readlane(z, f) - s.q0;
+            s.k0 = __builtin_amdgcn_readlane(ka, f);
+            s.nk = __builtin_amdgcn_readlane(kz, f) - s.k0;
+            s.local = tile - (readlane_u32(upto, f) - readlane_u32(n, f));
             return true;
         }
-        base += readlane_u32(upto, WAVE - 1);
+        base = readlane_u32(upto, WAVE - 1);
     }
     return false;
 }
 
-template <int HD, typename T>
-__global__ __launch_bounds__(PA_THREADS, (PromptShape<HD, T>::WAVES_PER_SIMD))
+template <int HD, typename T, int RW, int KG>
+__global__ __launch_bounds__(RW * KG * WAVE, (PromptShape<HD, T>::WAVES_PER_SIMD))
 void k_attn_prompt(PromptAttn p)
 {
     using S = PromptShape<HD, T>;
+    constexpr int ROWS = 32 * RW;
     constexpr int KT = S::KT, RB = S::RB, NSUB = KT / 32, ND = HD / 32;
     extern __shared__ __align__(16) uint8_t smem[];
 
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = wave % RW, kg = wave / RW;                   // wave of its key group
     const int col = lane & 31, h = lane >> 5;
 
     // ---- the block's tile, KV head and part ----------------------------------
@@ -122,27 +161,20 @@ void k_attn_prompt(PromptAttn p)
         kvh = blockIdx.x % nkv;
         tile = blockIdx.x / nkv;
     }
-    uint32_t seq, local;
-    if (!find_tile(p, tile, lane, seq, local)) return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    local = __builtin_amdgcn_readfirstlane(local);
-    const int32_t q0 = p.q_offsets[seq], nq = p.q_offsets[seq + 1] - q0;
-    const int32_t k0 = p.k_offsets[seq], k1 = p.k_offsets[seq + 1];
-    if (k0 < 0 || k1 < k0 || static_cast<uint32_t>(k1) > p.k_rows) {
-        if (threadIdx.x == 0) flag_range(p.err);
-        return;
-    }
-    const int32_t nk = k1 - k0, before = nk - nq;               // query i sees keys 0 .. i + before
+    PromptSeq seq;
+    if (!find_tile<ROWS>(p, tile, lane, seq)) return;
+    const int32_t q0 = seq.q0, nq = seq.nq, k0 = seq.k0, nk = seq.nk;
+    const int32_t before = nk - nq;                             // query i sees keys 0 .. i + before
     const uint32_t G = p.group, rows = static_cast<uint32_t>(nq) * G;
     // the longest tiles of a sequence first: what is left for the end of the launch is short
-    const uint32_t tiles = (rows + PA_ROWS - 1) / PA_ROWS;
-    const uint32_t r0 = (tiles - 1 - local) * PA_ROWS;
+    const uint32_t tiles = (rows + ROWS - 1) / ROWS;
+    const uint32_t r0 = (tiles - 1 - seq.local) * ROWS;
     const uint32_t r = r0 + wv * 32 + col;
     const bool live = r < rows;
     const uint32_t qi = min(r, rows - 1) / G, g = min(r, rows - 1) % G;
     const int32_t limit = live ? static_cast<int32_t>(qi) + before : -1;     // the row's last key
     // last key of the block, first and last key limits of the wave's rows
-    const int32_t blk_last = static_cast<int32_t>((min(r0 + PA_ROWS, rows) - 1) / G) + before;
+    const int32_t blk_last = static_cast<int32_t>((min(r0 + ROWS, rows) - 1) / G) + before;
     const uint32_t w0 = min(r0 + wv * 32, rows - 1), w1 = min(r0 + wv * 32 + 31, rows - 1);
     const bool wave_full = r0 + wv * 32 + 31 < rows;
     const int32_t wave_first = wave_full ? static_cast<int32_t>(w0 / G) + before : -1;
@@ -167,21 +199,37 @@ void k_attn_prompt(PromptAttn p)
     const uint64_t kb = p.k_stride * sizeof(T), vb = p.v_stride * sizeof(T);
     const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + static_cast<uint64_t>(k0) * kb + kvh * RB;
     const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + static_cast<uint64_t>(k0) * vb + kvh * RB;
+    uint8_t* mine = smem + kg * S::LDS;
     const uint32_t lds0 = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem));
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
+    constexpr int NI = S::TILE / 1024 / RW;
+    uint32_t koff[NI], voff[NI];                                // of a whole tile, from its first key
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+        const int at = (wv * NI + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
+        koff[u] = row * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row));
+        voff[u] = row * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row));
+    }
     auto issue = [&](int32_t t, int b) {
         const uint8_t* kt = kbase + static_cast<uint64_t>(t) * KT * kb;
         const uint8_t* vt = vbase + static_cast<uint64_t>(t) * KT * vb;
-        const int32_t last = nk - 1 - t * KT;                   // keys past the end: the last one again (masked)
-        constexpr int N = S::PER_WAVE / 2;
+        const uint32_t to = lds0 + b * 2 * S::TILE + wv * NI * 1024;
+        const int32_t last = nk - 1 - t * KT;
+        if (last >= KT - 1) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int at = (wv * N + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
-            const uint32_t src = static_cast<uint32_t>(min(row, last));
-            load_to_lds(kt, src * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row)),
-                        lds0 + b * 2 * S::TILE + (wv * N + u) * 1024);
-            load_to_lds(vt, src * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row)),
-                        lds0 + b * 2 * S::TILE + S::TILE + (wv * N + u) * 1024);
+            for (int u = 0; u < NI; ++u) {
+                load_to_lds(kt, koff[u], to + u * 1024);
+                load_to_lds(vt, voff[u], to + S::TILE + u * 1024);
+            }
+        } else {
+            // keys past the end: the last one again (masked)
+#pragma unroll
+            for (int u = 0; u < NI; ++u) {
+                const int at = (wv * NI + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
+                const uint32_t src = static_cast<uint32_t>(min(row, last));
+                load_to_lds(kt, src * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row)), to + u * 1024);
+                load_to_lds(vt, src * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row)), to + S::TILE + u * 1024);
+            }
         }
     };
 
@@ -194,38 +242,36 @@ void k_attn_prompt(PromptAttn p)
     const float c2 = p.scale_log2;
 
     auto tile_step = [&](int32_t t, int b) {
-        const uint8_t* kl = smem + b * 2 * S::TILE;
+        const uint8_t* kl = mine + b * 2 * S::TILE;
         const uint8_t* vl = kl + S::TILE;
         // ---- S^T = K Q^T ----
         f32x16_t s[NSUB];
 #pragma unroll
-        for (int u = 0; u < NSUB; ++u) {
+        for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < QN; ++ks) {
+        for (int ks = 0; ks < QN; ++ks)
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
                 const uint4 a = *reinterpret_cast<const uint4*>(kl + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col)));
                 if constexpr (S::F32) {
                     const f32x4v_t af = __builtin_bit_cast(f32x4v_t, a), bf = __builtin_bit_cast(f32x4v_t, qf[ks]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], s[u], 0, 0, 0);
-                } else if constexpr (__is_same(T, _Float16)) {
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
-                                                                  __builtin_bit_cast(f16x8_t, qf[ks]), s[u], 0, 0, 0);
                 } else {
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                                   __builtin_bit_cast(bf16x8_t, qf[ks]), s[u], 0, 0, 0);
+                    s[u] = mma16<T>(a, qf[ks], s[u]);
                 }
             }
-        }
         // ---- the causal mask: keys t KT + 32 u + 8 (i / 4) + 4 h + i % 4 ----
         if (t * KT + KT - 1 > wave_first) {
+            asm volatile("" : "+v"(s[0]));      // (a branch, not selects in every tile)
+            const int32_t room = limit - t * KT - 4 * h;
 #pragma unroll
             for (int u = 0; u < NSUB; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int32_t key = t * KT + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
-                    if (key > limit) s[u][i] = -INFINITY;
+                    if (32 * u + 8 * (i / 4) + i % 4 > room) s[u][i] = -INFINITY;
                 }
         }
         // ---- running maximum and sum ----
@@ -251,7 +297,7 @@ void k_attn_prompt(PromptAttn p)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c2, -mc));
-                sum += s[u][i];
+                if constexpr (S::F32) sum += s[u][i];
             }
         // ---- O^T += V^T P^T ----
         if constexpr (S::F32) {
@@ -279,6 +325,7 @@ void k_attn_prompt(PromptAttn p)
                 pb.y = pack2<T>(sv[o + 2], sv[o + 3]);
                 pb.z = pack2<T>(sv[o + 4], sv[o + 5]);
                 pb.w = pack2<T>(sv[o + 6], sv[o + 7]);
+                sum = add2<T>(pb.x, add2<T>(pb.y, add2<T>(pb.z, add2<T>(pb.w, sum))));
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const uint8_t* a = vl + (16 * ks + vrow) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
@@ -289,31 +336,56 @@ void k_attn_prompt(PromptAttn p)
                     const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 8 * RB));
                     typedef short s16x8_t __attribute__((ext_vector_type(8)));
                     const s16x8_t av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (__is_same(T, _Float16))
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, av),
-                                                                        __builtin_bit_cast(f16x8_t, pb), acc[d], 0, 0, 0);
-                    else
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av),
-                                                                         __builtin_bit_cast(bf16x8_t, pb), acc[d], 0, 0, 0);
+                    acc[d] = mma16<T>(__builtin_bit_cast(uint4, av), pb, acc[d]);
                 }
             }
         }
     };
 
-    if (t0 < t1) issue(t0, 0);
-    for (int32_t t = t0; t < t1; ++t) {
-        const int b = (t - t0) & 1;
+    // group kg takes tiles t0 + kg, t0 + kg + KG, ..
+    if (t0 + kg < t1) issue(t0 + kg, 0);
+    // The query loads end here: the compiler, which does not count the direct loads, would
+    // otherwise wait for them at their use in the loop, and so for the next tile on its way.
+#pragma unroll
+    for (int s = 0; s < QN; ++s) asm volatile("" : "+v"(qf[s].x), "+v"(qf[s].y), "+v"(qf[s].z), "+v"(qf[s].w));
+    int b = 0;
+    for (int32_t tt = t0; tt < t1; tt += KG, b ^= 1) {
+        const int32_t t = tt + kg;
         // this wave's part of tile t has arrived and its reads of the other buffer are done; after
         // the barrier so are every wave's
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (t + 1 < t1) issue(t + 1, b ^ 1);
-        if (t * KT <= wave_last) tile_step(t, b);
+        if (t + KG < t1) issue(t + KG, b ^ 1);
+        if (t * KT <= min(wave_last, t1 * KT - 1)) tile_step(t, b);
+    }
+    sum = half_sum(sum);
+
+    // ---- the second key group's part joins the first's, lane by lane ---------------
+    if constexpr (KG == 2) {
+        float* other = reinterpret_cast<float*>(smem) + wv * (ND * 16 + 2) * WAVE + lane;
+        __syncthreads();                                        // (every tile is read)
+        if (kg == 1) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) other[(d * 16 + i) * WAVE] = acc[d][i];
+            other[ND * 16 * WAVE] = mx;
+            other[(ND * 16 + 1) * WAVE] = sum;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = other[ND * 16 * WAVE], mn = fmaxf(mx, m1), m0 = mn > -INFINITY ? mn : 0.f;
+        const float f0 = __builtin_amdgcn_exp2f((mx - m0) * c2), f1 = __builtin_amdgcn_exp2f((m1 - m0) * c2);
+        sum = sum * f0 + other[(ND * 16 + 1) * WAVE] * f1;
+        mx = mn;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * f0 + other[(d * 16 + i) * WAVE] * f1;
     }
 
     // ---- the result -----------------------------------------------------------
-    sum = half_sum(sum);
     if (!live) return;
     const size_t row_out = static_cast<size_t>(q0) + qi;
     if (p.splits == 1) {
@@ -349,12 +421,12 @@ void k_attn_prompt(PromptAttn p)
 
 // one wave per (query row, head) of the sequences
 template <int HD, typename T>
-__global__ __launch_bounds__(PA_THREADS)
+__global__ __launch_bounds__(JOIN_WAVES * WAVE)
 void k_prompt_join(PromptAttn p)
 {
     const int lane = threadIdx.x & 63;
     const uint32_t heads = p.num_kv_heads * p.group;
-    const uint32_t w = blockIdx.x * PA_WAVES + (threadIdx.x >> 6), row = w / heads;
+    const uint32_t w = blockIdx.x * JOIN_WAVES + (threadIdx.x >> 6), row = w / heads;
     if (row >= p.q_rows || static_cast<int32_t>(row) < p.q_offsets[0] ||
         static_cast<int32_t>(row) >= p.q_offsets[p.n_seqs])
         return;
@@ -364,16 +436,39 @@ void k_prompt_join(PromptAttn p)
     store_row<HD>(static_cast<T*>(p.out) + row * p.out_stride + (w % heads) * HD, o, lane);
 }
 
+// Which form, by the blocks that a call gives and the key tiles of its longest sequence (8 query heads a KV
+// head, 4 KV heads, head_dim 128, bf16; us of the kernel, and of the join where there is one):
+//   2 x 2 waves (64 rows, two key groups: one block a CU, half the chain of tiles) while 64-row blocks leave
+//     CUs idle: 512 tokens 11.9 against 16.0 (4 x 1) and 15.1 (4 x 2);
+//   4 x 2 (128 rows) up to two such blocks a CU: 1024 tokens 24.4 / 27.0 / 26.4, 2048 53.8 / 57.5 / 77, unless
+//     there are few tiles to share out;
+//   4 x 1 beyond (two blocks a CU, nothing to merge): 4096 tokens 165 / 175 / 255, 64 sequences of 64 24 / 39 / 50.
+// Keys are split over blocks (each part eight tiles or more) until every CU has one: 64 tokens behind 8000 take
+// 101 in one part of 2 x 2 and 21 + 4 in eight; over long parts 4 x 2 is ahead again (256 tokens behind 4000:
+// 30 + 5 in four parts against 36 + 4 in two of 2 x 2).
 void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k)
 {
-    a.tiles = static_cast<uint32_t>(static_cast<uint64_t>(a.q_rows) * a.group / PA_ROWS) + a.n_seqs;
-    const uint32_t kt = type == SMOE_TYPE_F32 || head_dim == 256 ? 32 : 64;
+    constexpr uint64_t CUS = 256;
+    const bool f32 = type == SMOE_TYPE_F32, wide = head_dim == 256;
+    const uint32_t kt = f32 || wide ? 32 : 64, keys = max_k / kt + (max_k % kt != 0);
     // full tiles alone: a part-filled one of each sequence may not exist
-    const uint64_t blocks = std::max<uint64_t>(
-        1, (static_cast<uint64_t>(a.q_rows) * a.group + PA_ROWS - 1) / PA_ROWS * a.num_kv_heads);
-    const uint32_t want = static_cast<uint32_t>(std::min<uint64_t>(JOIN_MAX, 512 / blocks));
-    // a part has four tiles or more
-    a.splits = std::max<uint32_t>(1, std::min<uint32_t>(want, max_k / (4 * kt)));
+    const uint64_t rows = static_cast<uint64_t>(a.q_rows) * a.group;
+    const uint64_t b64 = (rows + 63) / 64 * a.num_kv_heads, b128 = (rows + 127) / 128 * a.num_kv_heads;
+    auto parts = [&](uint64_t blocks) {
+        return static_cast<uint32_t>(std::max<uint64_t>(
+            1, std::min<uint64_t>({CUS / std::max<uint64_t>(blocks, 1), JOIN_MAX, keys / 8})));
+    };
+    // (LDS and registers of a CU: head_dim 256 has room for one group of four waves, or in 16 bits two of two)
+    if (!(f32 && wide) && b64 <= CUS && (wide || keys <= 24 * parts(b64))) {
+        a.row_waves = 2;
+        a.key_groups = 2;
+        a.splits = parts(b64);
+    } else {
+        a.row_waves = 4;
+        a.key_groups = !wide && keys >= 4 && (b128 <= CUS || (b128 <= 2 * CUS && keys >= 8)) ? 2 : 1;
+        a.splits = parts(b128);
+    }
+    a.tiles = static_cast<uint32_t>(rows / (32 * a.row_waves)) + a.n_seqs;
 }
 
 size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t head_dim)
@@ -382,27 +477,42 @@ size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t head_dim)
     return part_floats(static_cast<size_t>(a.q_rows) * a.num_kv_heads * a.group, a.splits, head_dim) * sizeof(float);
 }
 
+template <int HD, typename T, int RW, int KG>
+static hipError_t launch_prompt(const PromptAttn& a, dim3 grid, hipStream_t s)
+{
+    constexpr uint32_t lds = KG * PromptShape<HD, T>::LDS;
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    if constexpr (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_prompt<HD, T, RW, KG>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    launch_kernel_lds(k_attn_prompt<HD, T, RW, KG>, grid, dim3(RW * KG * WAVE), lds, s, a);
+    return hipGetLastError();
+}
+
 hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t head_dim, uint32_t type, hipStream_t s)
 {
     return with_type_and_head(type, head_dim, [&](auto t, auto hd) {
         constexpr int HD = decltype(hd)::value;
         using T = decltype(t);
-        constexpr uint32_t lds = PromptShape<HD, T>::LDS;
-        static_assert(lds <= 160 * 1024, "LDS of a CU");
-        if constexpr (lds > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_prompt<HD, T>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e != hipSuccess) return e;
-        }
         // every XCD has as many blocks of a tile row where KV heads share or split XCDs
         const uint32_t nkv = a.num_kv_heads;
         const uint32_t per = 8 % nkv == 0 ? 8 / nkv : 1;
-        const uint32_t blocks = (a.tiles + per - 1) / per * per * nkv;
-        launch_kernel_lds(k_attn_prompt<HD, T>, dim3(blocks, a.splits), dim3(PA_THREADS), lds, s, a);
-        if (a.splits > 1) {
-            const uint32_t waves = a.q_rows * nkv * a.group;
-            launch_kernel(k_prompt_join<HD, T>, dim3((waves + PA_WAVES - 1) / PA_WAVES), dim3(PA_THREADS), s, a);
+        const dim3 grid((a.tiles + per - 1) / per * per * nkv, a.splits);
+        hipError_t e;
+        if (a.key_groups == 1) {
+            e = launch_prompt<HD, T, 4, 1>(a, grid, s);
+        } else if (a.row_waves == 2) {
+            if constexpr (2 * PromptShape<HD, T>::LDS <= 160 * 1024) e = launch_prompt<HD, T, 2, 2>(a, grid, s);
+            else e = hipErrorInvalidValue;
+        } else {
+            if constexpr (PromptShape<HD, T>::WAVES_PER_SIMD == 2) e = launch_prompt<HD, T, 4, 2>(a, grid, s);
+            else e = hipErrorInvalidValue;
         }
+        if (e != hipSuccess || a.splits == 1) return e;
+        const uint32_t waves = a.q_rows * nkv * a.group;
+        launch_kernel(k_prompt_join<HD, T>, dim3((waves + JOIN_WAVES - 1) / JOIN_WAVES), dim3(JOIN_WAVES * WAVE), s, a);
         return hipGetLastError();
     });
 }
