@@ -127,66 +127,113 @@ hipError_t launch_qk_rows(const QkRows& a, uint32_t head_dim, uint32_t type, hip
 // ---------------------------------------------------------------------------
 // the 4-bit cache: a wave takes some groups of one row
 // ---------------------------------------------------------------------------
+// what the call says of 64 sequences, one a lane
+struct CallSeqs {
+    int32_t first, end, start, slot;                       // rows first .. end - 1, position of the first, slot
+};
+__device__ __forceinline__ CallSeqs load_seqs(const Kv4Rows& p, uint32_t i, int lane)
+{
+    const uint32_t b = min(i + lane, p.n_seqs - 1);
+    CallSeqs s;
+    s.first = p.offsets ? p.offsets[b] : static_cast<int32_t>(b);
+    s.end = p.offsets ? p.offsets[b + 1] : static_cast<int32_t>(b) + 1;
+    s.start = p.start[b];
+    s.slot = p.slots ? p.slots[b] : static_cast<int32_t>(b);
+    if (i + lane >= p.n_seqs) s.end = s.first;
+    return s;
+}
+
 struct CachePlace {
     uint32_t slot, pos;
     bool in_seq, ok;       // the row is of a sequence; its place is in the cache
+    bool later;            // a later sequence of the call names the same place
 };
-
-// Sequence, slot and position of a row, by the whole wave.
-__device__ __forceinline__ CachePlace place_of_row(const Kv4Rows& p, uint32_t row, int lane, uint32_t& seq, int32_t& at)
+// Sequence, slot and position of a row, by the whole wave; `near` holds the 64 sequences from i0 on.
+__device__ __forceinline__ CachePlace place_of_row(const Kv4Rows& p, uint32_t row, int lane)
 {
     CachePlace c{};
-    seq = row;
-    at = 0;
-    c.in_seq = true;
-    if (p.offsets) {
-        // the sequences that end at or before the row come before its own
-        uint32_t before = 0;
-        for (uint32_t i = 0; i < p.n_seqs; i += WAVE) {
-            const bool ends = i + lane < p.n_seqs && p.offsets[i + lane + 1] <= static_cast<int32_t>(row);
-            const uint32_t n = __popcll(__ballot(ends));
-            before += n;
-            if (n < WAVE) break;
+    uint32_t seq = 0;
+    // (without offsets row r is sequence r's)
+    for (uint32_t i = p.offsets ? 0u : row / WAVE * WAVE; i < p.n_seqs; i += WAVE) {
+        const CallSeqs s = load_seqs(p, i, lane);
+        if (!c.in_seq) {
+            // the first sequence that ends behind the row
+            const uint64_t after = __ballot(s.end > static_cast<int32_t>(row) && i + lane < p.n_seqs);
+            if (!after) continue;
+            const int f = __ffsll(static_cast<unsigned long long>(after)) - 1;
+            seq = i + f;
+            const int32_t at = static_cast<int32_t>(row) - __builtin_amdgcn_readlane(s.first, f);
+            if (at < 0) return c;
+            c.in_seq = true;
+            c.slot = __builtin_amdgcn_readlane(s.slot, f);
+            c.pos = static_cast<uint32_t>(__builtin_amdgcn_readlane(s.start, f)) + static_cast<uint32_t>(at);
+            c.ok = c.slot < p.c.n_slots && c.pos < p.c.capacity;
+            if (!c.ok) {
+                if (lane == 0) flag_range(p.err);
+                return c;
+            }
+            if (!p.slots) return c;
         }
-        seq = before;
-        c.in_seq = seq < p.n_seqs && p.offsets[seq] <= static_cast<int32_t>(row);
-        if (!c.in_seq) return c;
-        at = static_cast<int32_t>(row) - p.offsets[seq];
+        // (a lane without a sequence of its own has first = end)
+        c.later = __ballot(i + lane > seq && static_cast<uint32_t>(s.slot) == c.slot &&
+                           c.pos - static_cast<uint32_t>(s.start) < static_cast<uint32_t>(s.end - s.first)) != 0;
+        if (c.later) return c;
     }
-    const int64_t slot = p.slots ? static_cast<int64_t>(p.slots[seq]) : static_cast<int64_t>(seq);
-    const int64_t pos = static_cast<int64_t>(p.start[seq]) + at;
-    c.ok = slot >= 0 && slot < p.c.n_slots && pos >= 0 && pos < p.c.capacity;
-    if (!c.ok) {
-        if (lane == 0) flag_range(p.err);
-        return c;
-    }
-    c.slot = static_cast<uint32_t>(slot);
-    c.pos = static_cast<uint32_t>(pos);
     return c;
 }
 
-// whether a later sequence of the call writes the same place (a slot named twice)
-__device__ __forceinline__ bool written_later(const Kv4Rows& p, const CachePlace& c, uint32_t seq, int lane)
+// eight lanes' group of 64 values to its place
+template <int HD>
+__device__ __forceinline__ void store_group(const Kv4Rows& p, const CachePlace& c, uint32_t side, uint32_t hg, int lane,
+                                            const float (&x)[8])
 {
-    if (!p.slots) return false;
-    for (uint32_t i = seq + 1; i < p.n_seqs; i += WAVE) {
-        const uint32_t b = i + lane;
-        bool same = b < p.n_seqs && p.slots[b] == static_cast<int32_t>(c.slot);
-        if (same) {
-            const int64_t n = p.offsets ? static_cast<int64_t>(p.offsets[b + 1]) - p.offsets[b] : 1;
-            const int64_t d = static_cast<int64_t>(c.pos) - p.start[b];
-            same = d >= 0 && d < n;
-        }
-        if (__ballot(same)) return true;
+    constexpr uint32_t NG = HD / 64;
+    const uint32_t head = hg / NG, part = hg % NG;
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+        lo = fminf(lo, x[j]);
+        hi = fmaxf(hi, x[j]);
     }
-    return false;
+    lo = seg8_min(lo);
+    hi = -seg8_min(-hi);
+    const float span = (hi - lo) / 15.0f;
+    uint32_t sb = __builtin_bit_cast(uint16_t, static_cast<__bf16>(span));
+    if ((sb & 0x7FFFu) == 0) sb = 0x3F80u;                     // a constant group: scale 1
+    const uint32_t mb = __builtin_bit_cast(uint16_t, static_cast<__bf16>(lo));
+    const float s = bf16_to_f32(sb), m = bf16_to_f32(mb);
+    // code = rint((x - m) / s), the difference and the quotient each rounded.  The quotient by s's reciprocal r:
+    // one step makes r the rounded 1 / s (checked for all 128 mantissas that a bf16 scale has, from any first r
+    // within two steps), and with that q + (d - q s) r is the rounded d / s (Markstein), in three operations
+    // instead of a division's two dozen.  Scales near the ends of the range divide.
+    uint32_t word = 0;
+    if (s > 0x1p-100f && s < 0x1p100f) {
+        float r = __builtin_amdgcn_rcpf(s);
+        r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = x[j] - m, q = d * r;
+            const float c0 = rintf(__builtin_fmaf(__builtin_fmaf(-q, s, d), r, q));
+            word |= static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(c0, 0.f), 15.f))) << (4 * j);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float q = x[j] - m;
+            q = q / s;
+            word |= static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(q), 0.f), 15.f))) << (4 * j);
+        }
+    }
+    const size_t line = (static_cast<size_t>(c.slot) * p.c.num_kv_heads + head) * p.c.capacity + c.pos;
+    reinterpret_cast<uint32_t*>(p.c.codes[side] + line * (HD / 2) + part * 32)[lane & 7] = word;
+    if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(p.c.params[side])[line * NG + part] = sb | (mb << 16);
 }
 
 template <int HD, typename T>
 __global__ __launch_bounds__(RW_THREADS)
 void k_kv4_append(Kv4Rows p, uint32_t gpw, uint32_t waves_per_row)
 {
-    constexpr uint32_t NG = HD / 64;                           // groups of a head
+    constexpr uint32_t NG = HD / 64, STEP = WAVE / 8;          // eight lanes a group, eight groups a step
     const int lane = threadIdx.x & 63;
     const uint32_t w = blockIdx.x * RW_WAVES + (threadIdx.x >> 6), row = w / waves_per_row;
     if (p.lens_out && blockIdx.x == 0) {
@@ -196,41 +243,23 @@ void k_kv4_append(Kv4Rows p, uint32_t gpw, uint32_t waves_per_row)
     if (row >= p.n_rows) return;
     const uint32_t per_side = p.c.num_kv_heads * NG, groups = 2 * per_side;
     const uint32_t g0 = w % waves_per_row * gpw, g1 = min(g0 + gpw, groups);
-    uint32_t seq;
-    int32_t at;
-    const CachePlace c = place_of_row(p, row, lane, seq, at);
-    if (!c.ok || written_later(p, c, seq, lane)) return;
-    // eight lanes a group, eight groups a step
-    for (uint32_t g = g0 + (lane >> 3); g < g1; g += WAVE / 8) {
-        const uint32_t side = g / per_side, hg = g % per_side, head = hg / NG, part = hg % NG;
-        float x[8];
+    auto load = [&](uint32_t g, float (&x)[8]) {
+        const uint32_t side = g >= per_side, hg = g - side * per_side;
         load8(static_cast<const T*>(p.rows[side]) + row * p.stride[side] + hg * 64 + (lane & 7) * 8, x);
-        float lo = x[0], hi = x[0];
+    };
+    uint32_t g = g0 + (lane >> 3);
+    float x[8];
+    if (g < g1) load(g, x);                                    // (requested before its place is known)
+    const CachePlace c = place_of_row(p, row, lane);
+    if (!c.ok || c.later) return;
+    while (g < g1) {
+        float y[8];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) {
-            lo = fminf(lo, x[j]);
-            hi = fmaxf(hi, x[j]);
-        }
-        lo = seg8_min(lo);
-        hi = -seg8_min(-hi);
-        const float span = (hi - lo) / 15.0f;
-        uint32_t sb = __builtin_bit_cast(uint16_t, static_cast<__bf16>(span));
-        if ((sb & 0x7FFFu) == 0) sb = 0x3F80u;                 // a constant group: scale 1
-        const uint32_t mb = __builtin_bit_cast(uint16_t, static_cast<__bf16>(lo));
-        const float s = bf16_to_f32(sb), m = bf16_to_f32(mb);
-        uint32_t word = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // two separately rounded operations: (x - m), then / s
-            float q = x[j] - m;
-            q = q / s;
-            int code = static_cast<int>(rintf(q));
-            code = code < 0 ? 0 : (code > 15 ? 15 : code);
-            word |= static_cast<uint32_t>(code) << (4 * j);
-        }
-        const size_t line = (static_cast<size_t>(c.slot) * p.c.num_kv_heads + head) * p.c.capacity + c.pos;
-        reinterpret_cast<uint32_t*>(p.c.codes[side] + line * (HD / 2) + part * 32)[lane & 7] = word;
-        if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(p.c.params[side])[line * NG + part] = sb | (mb << 16);
+        for (int j = 0; j < 8; ++j) y[j] = x[j];
+        if (g + STEP < g1) load(g + STEP, x);
+        const uint32_t side = g >= per_side;
+        store_group<HD>(p, c, side, g - side * per_side, lane, y);
+        g += STEP;
     }
 }
 
@@ -238,18 +267,16 @@ template <int HD, typename T>
 __global__ __launch_bounds__(RW_THREADS)
 void k_kv4_read(Kv4Rows p, uint32_t gpw, uint32_t waves_per_row)
 {
-    constexpr uint32_t NG = HD / 64;
+    constexpr uint32_t NG = HD / 64, STEP = WAVE / 8;
     const int lane = threadIdx.x & 63;
     const uint32_t w = blockIdx.x * RW_WAVES + (threadIdx.x >> 6), row = w / waves_per_row;
     if (row >= p.n_rows) return;
     const uint32_t per_side = p.c.num_kv_heads * NG, groups = 2 * per_side;
     const uint32_t g0 = w % waves_per_row * gpw, g1 = min(g0 + gpw, groups);
-    uint32_t seq;
-    int32_t at;
-    const CachePlace c = place_of_row(p, row, lane, seq, at);
+    const CachePlace c = place_of_row(p, row, lane);
     if (!c.in_seq) return;                                     // rows behind the last sequence stay
-    for (uint32_t g = g0 + (lane >> 3); g < g1; g += WAVE / 8) {
-        const uint32_t side = g / per_side, hg = g % per_side, head = hg / NG, part = hg % NG;
+    for (uint32_t g = g0 + (lane >> 3); g < g1; g += STEP) {
+        const uint32_t side = g >= per_side, hg = g - side * per_side, head = hg / NG, part = hg % NG;
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = 0.f;                // a place outside the cache reads as zeros
@@ -279,7 +306,8 @@ hipError_t launch_kv4_append(const Kv4Rows& a, uint32_t head_dim, uint32_t type,
         constexpr int HD = decltype(hd)::value;
         uint32_t gpw;
         const uint32_t per_row = row_waves(a.n_rows, 2 * a.c.num_kv_heads * (HD / 64), gpw);
-        launch_kernel(k_kv4_append<HD, decltype(t)>, row_grid(a.n_rows, per_row), dim3(RW_THREADS), s, a, gpw, per_row);
+        const dim3 grid = a.n_rows ? row_grid(a.n_rows, per_row) : dim3(1);   // (no rows: the lengths alone)
+        launch_kernel(k_kv4_append<HD, decltype(t)>, grid, dim3(RW_THREADS), s, a, gpw, per_row);
         return hipGetLastError();
     });
 }
