@@ -430,7 +430,9 @@ int smoe_hip_attention_layer(SmoeMetalCtx* ctx, const SmoeAttnLayerArgs* args);
  * rules of this section:
  *   - type: the element type of a call's rows (SMOE_TYPE_*).  Sums, softmax
  *     and norms are fp32 (16-bit types: the softmax weights are rounded to the
- *     type before they meet V); results are rounded once;
+ *     type before they meet V; f32 prompts and the 4-bit cache: the products
+ *     take their operands as two f16, 22 bits of each value); results are
+ *     rounded once;
  *   - rows lie a stride (elements) apart, heads side by side in a row.  Rows
  *     are 16-byte aligned and their strides multiples of 16 bytes, up to 2^22
  *     elements, so q, k and v may be column ranges of one matrix;
@@ -442,7 +444,8 @@ int smoe_hip_attention_layer(SmoeMetalCtx* ctx, const SmoeAttnLayerArgs* args);
  *   - offsets, slots, positions and lengths live on the device.  One that
  *     points outside its buffer is never followed: the call skips or zeroes
  *     what it concerns and the next smoe_hip_synchronize returns SMOE_ERR_ARG;
- *   - scratch (parts of split keys) grows outside graph capture; under capture
+ *   - scratch (parts of split keys, the f16 halves of a f32 prompt's k and v:
+ *     as many bytes as they have) grows outside graph capture; under capture
  *     a call needs that of an earlier call of the same sizes, else
  *     SMOE_ERR_CAPTURE.  The calls of a context share it: calls, and replays
  *     of graphs captured from it, that may run at the same time need contexts
@@ -481,7 +484,9 @@ int smoe_hip_qk_norm_rope(SmoeMetalCtx* ctx, const SmoeQkRowsArgs* args);
  * head_dim]; k_offsets NULL: q_offsets.  max_k: keys of the longest sequence as
  * far as known, 0: k_rows; it only decides how the work is split.  out must not
  * overlap the inputs.  The weight of a key that a query does not see is exactly
- * 0, so v has to be finite wherever another query of the sequence sees it. */
+ * 0, so v has to be finite wherever another query of the sequence sees it.  f32: a
+ * value of k or v is taken to 2^-22 of itself or 2^-38 of the largest of its KV
+ * head's values in the 32 keys it shares a tile with, whichever is more. */
 typedef struct {
     const void*    q;
     const void*    k;

@@ -228,8 +228,11 @@ extern "C" int smoe_hip_attention_prompt(SmoeMetalCtx* ctx, const SmoePromptAttn
     p.scale_log2 = a->scale * 1.44269504088896341f;
     p.err = v.err;
     smoe::prompt_plan(p, a->head_dim, a->type, a->max_k ? a->max_k : a->k_rows);
-    if (const size_t need = smoe::prompt_scratch_bytes(p, a->head_dim))
-        if (const int rc = smoe::context_attention_scratch(ctx, need, &p.part)) return rc;
+    if (const size_t need = smoe::prompt_scratch_bytes(p, a->head_dim)) {
+        float* scratch = nullptr;
+        if (const int rc = smoe::context_attention_scratch(ctx, need, &scratch)) return rc;
+        smoe::prompt_scratch(p, a->head_dim, scratch);
+    }
     return launch(ctx, SMOE_KERNEL_ATTENTION_PROMPT, "attention_prompt", v.stream, smoe::launch_attention_prompt, p,
                   a->head_dim, a->type);
 }

@@ -76,11 +76,15 @@ struct PromptAttn {
     uint32_t key_groups;        // groups of such waves that take the tile's keys in turn
     uint32_t splits;            // parts of a sequence's keys, joined by a second launch
     float* part;                // rows = query rows times heads (part_floats)
+    uint32_t plane_tiles;       // f32: tiles of 32 keys, at most, that share a power of two; else 0
+    uint16_t* planes;           // f32: K hi, K lo, V hi, V lo [k_rows][KV heads][head_dim] f16
+    int2* powers;               // f32: [KV heads][plane_tiles] powers of K and of V
     uint32_t* err;
 };
 // tiles and splits of a call (max_k: the longest sequence's keys as far as the caller knows), and its scratch
 void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k);
 size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t head_dim);
+void prompt_scratch(PromptAttn& a, uint32_t head_dim, void* scratch);
 hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t head_dim, uint32_t type, hipStream_t s);
 
 // attention of one token a sequence over the 4-bit cache (attn_kv4.hip); strides in elements

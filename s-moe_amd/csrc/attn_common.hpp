@@ -62,6 +62,16 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8])
     }
 }
 
+// x = hi + lo in f16
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    const f16x2_t hv = __builtin_bit_cast(f16x2_t, hi);
+    const auto l = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hv.x), b - static_cast<float>(hv.y));
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
 // maximum / sum of the values of lanes l and l ^ 32
 __device__ __forceinline__ float half_max(float v)
 {

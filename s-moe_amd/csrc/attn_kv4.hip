@@ -59,16 +59,6 @@ __device__ __forceinline__ f16x8_t codes8(uint32_t w, uint32_t even, uint32_t od
 // place j of codes8 holds code code_at(j)
 __device__ constexpr int code_at(int j) { return (j >> 1) + 4 * (j & 1); }
 
-// x = hi + lo in f16
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo)
-{
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    hi = __builtin_bit_cast(uint32_t, h);
-    const f16x2_t hv = __builtin_bit_cast(f16x2_t, hi);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hv.x), b - static_cast<float>(hv.y));
-    lo = __builtin_bit_cast(uint32_t, l);
-}
-
 // maximum / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float quads_max(float v)
 {

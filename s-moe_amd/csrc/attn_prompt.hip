@@ -19,14 +19,25 @@
 //     read in that key order).  The rows' only exchange is between lanes l and l ^ 32.
 //     Tiles.  K and V tiles go to LDS by direct loads, one tile ahead, in 16-byte
 //     pieces whose place in a row is exchanged (kswz, vswz) so that the operand reads
-//     meet no bank twice: K as 16-byte pieces of 32 rows, V (16 bits) by transposing
-//     reads of 8 rows, V (32 bits) as dwords.
-//     f32 runs on v_mfma_f32_32x32x2_f32 throughout, 16-bit types on
-//     v_mfma_f32_32x32x16 with P rounded to their type (their sums are of the
-//     unrounded P, in fp32).
+//     meet no bank twice: K as 16-byte pieces of 32 rows, V by transposing reads of 8 rows.
+//     16-bit types: v_mfma_f32_32x32x16 with P rounded to their type (the weights' sum is
+//     of the rounded ones, in fp32).  f32: every operand as two f16 (hi + lo, 22 bits) and
+//     three products for one, 16 / 3 times the rate of the fp32 MFMA.  K and V are split
+//     by k_prompt_planes, at a power of two for 32 keys, Q here (one for a row), P here at
+//     2^15 and the V tile's power against the smallest so far.
+//     One accumulator takes the three: no cancellation sets them apart.
+//     Bound: large calls by the matrix cores at the clock that the power limit leaves
+//     (64 query heads of 128 on 4, 8192 tokens, bf16: 1.10 ms, 1.0 PF/s of causal products;
+//     without its softmax 0.98 ms; a large matrix product reaches 1.2 PF/s), small ones by
+//     launch, tile search and first loads (~6 us) and one wave a SIMD.  f32, 32 heads on 4:
+//     4096 tokens 424 us, 512 tokens 23 us after 4 us of k_prompt_planes; on the fp32 MFMA
+//     45 us at 512.
+//   k_prompt_planes the f16 planes of f32 K and V: one read, one write (64 MB at 5 TB/s; 3 to
+//     4 us for the few blocks of a short prompt).
 //   k_prompt_join   where the keys were split: the parts of each row rescaled to
 //     their common maximum and normalised.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.hpp"
 #include "kernels.hpp"
@@ -38,19 +49,17 @@ constexpr int JOIN_WAVES = 4;
 template <int HD, typename T>
 struct PromptShape {
     static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int PLANES = F32 ? 2 : 1;                 // f16 matrices that K, and V, are read as
     static constexpr int KT = F32 || HD == 256 ? 32 : 64;      // keys of a tile
-    static constexpr int RB = HD * static_cast<int>(sizeof(T));  // bytes of a K or V row
-    static constexpr int CPR = RB / 16;                          // 16-byte pieces of a row
-    static constexpr int TILE = KT * RB;                         // bytes of a K or V tile
-    static constexpr int LDS = 4 * TILE;                         // two tiles each of K and V
+    static constexpr int RB = 2 * HD;                            // bytes of a row
+    static constexpr int TILE = KT * RB;                         // bytes of a plane's tile
+    static constexpr int BUF = 2 * PLANES * TILE;                // K planes, then V planes
+    static constexpr int LDS = 2 * BUF;                          // of a key group
     static constexpr int WAVES_PER_SIMD = HD == 256 ? 1 : 2;
     // piece c of row r stands at piece c ^ kswz(r) (K), c ^ vswz(r) (V): the rows that one
     // pass of an operand read touches then lie in different banks of the 256-byte width
     __host__ __device__ static constexpr int kswz(int r) { return RB >= 256 ? (r & 15) : ((r >> 1) & 7); }
-    __host__ __device__ static constexpr int vswz(int r)
-    {
-        return F32 ? ((r >> 2) & 1) << 3 : RB >= 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
-    }
+    __host__ __device__ static constexpr int vswz(int r) { return RB >= 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 };
 
 // lane l's 16 bytes at base + off (off per lane) land at LDS byte address lds + 16 l
@@ -69,6 +78,15 @@ __device__ __forceinline__ f32x16_t mma16(uint4 a, uint4 b, f32x16_t c)
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
                                                        c, 0, 0, 0);
+}
+// transposing reads at `at` and eight rows on: this lane's values of four rows each
+__device__ __forceinline__ uint4 read_rows8(const uint8_t* at, int row_bytes)
+{
+    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * row_bytes));
+    return __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 // the two values of w added to c
 template <typename T>
@@ -100,35 +118,134 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
 struct PromptSeq {
     int32_t q0, nq, k0, nk;
     uint32_t local;                             // tile of the sequence
+    uint32_t ktile;                             // first key tile of the sequence, of PLANE_KEYS each
 };
+// what one lane knows of a sequence
+struct PromptLane {
+    int32_t a, z, ka, kz;
+    bool ok;
+};
+__device__ __forceinline__ PromptLane load_seq(const PromptAttn& p, uint32_t i, int lane)
+{
+    const uint32_t b = min(i + lane, p.n_seqs - 1);
+    PromptLane s{p.q_offsets[b], p.q_offsets[b + 1], p.k_offsets[b], p.k_offsets[b + 1], false};
+    s.ok = i + lane < p.n_seqs && s.a >= 0 && s.z >= s.a && static_cast<uint32_t>(s.z) <= p.q_rows && s.ka >= 0 &&
+           s.kz >= s.ka && static_cast<uint32_t>(s.kz) <= p.k_rows;
+    return s;
+}
+constexpr int NO_POWER = 200;                   // of V values that are all 0
+constexpr int PLANE_KEYS = 32;                  // keys that share a power of two in the f16 planes of f32 rows
+// (a sequence without queries has none)
+__device__ __forceinline__ uint32_t plane_tiles(const PromptLane& s)
+{
+    return s.ok && s.z > s.a ? (static_cast<uint32_t>(s.kz - s.ka) + PLANE_KEYS - 1) / PLANE_KEYS : 0;
+}
 template <int ROWS>
 __device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, PromptSeq& s)
 {
-    uint32_t base = 0;
+    uint32_t base = 0, kbase = 0;
     for (uint32_t i = 0; i < p.n_seqs; i += WAVE) {
-        const uint32_t b = min(i + lane, p.n_seqs - 1);
-        const int32_t a = p.q_offsets[b], z = p.q_offsets[b + 1], ka = p.k_offsets[b], kz = p.k_offsets[b + 1];
-        const bool ok = a >= 0 && z >= a && static_cast<uint32_t>(z) <= p.q_rows && ka >= 0 && kz >= ka &&
-                        static_cast<uint32_t>(kz) <= p.k_rows;
-        uint32_t n = 0;
-        if (i + lane < p.n_seqs) {
-            if (ok) n = (static_cast<uint32_t>(z - a) * p.group + ROWS - 1) / ROWS;
-            else if (tile == 0) flag_range(p.err);
-        }
-        const uint32_t upto = base + wave_scan(n);
+        const PromptLane l = load_seq(p, i, lane);
+        if (tile == 0 && i + lane < p.n_seqs && !l.ok) flag_range(p.err);
+        const uint32_t n = l.ok ? (static_cast<uint32_t>(l.z - l.a) * p.group + ROWS - 1) / ROWS : 0, kn = plane_tiles(l);
+        const uint32_t upto = base + wave_scan(n), kupto = kbase + wave_scan(kn);
         const uint64_t past = __ballot(upto > tile);
         if (past) {
             const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            s.q0 = __builtin_amdgcn_readlane(a, f);
-            s.nq = __builtin_amdgcn_readlane(z, f) - s.q0;
-            s.k0 = __builtin_amdgcn_readlane(ka, f);
-            s.nk = __builtin_amdgcn_readlane(kz, f) - s.k0;
+            s.q0 = __builtin_amdgcn_readlane(l.a, f);
+            s.nq = __builtin_amdgcn_readlane(l.z, f) - s.q0;
+            s.k0 = __builtin_amdgcn_readlane(l.ka, f);
+            s.nk = __builtin_amdgcn_readlane(l.kz, f) - s.k0;
             s.local = tile - (readlane_u32(upto, f) - readlane_u32(n, f));
+            s.ktile = readlane_u32(kupto, f) - readlane_u32(kn, f);
             return true;
         }
         base = readlane_u32(upto, WAVE - 1);
+        kbase = readlane_u32(kupto, WAVE - 1);
     }
     return false;
+}
+
+// ---------------------------------------------------------------------------
+// f32 rows of K and V as f16 planes: x 2^e = hi + lo to 22 bits, e the power of two that
+// brings the largest finite value of 32 keys (of one KV head, K or V) to 2^13 .. 2^14
+// ---------------------------------------------------------------------------
+// exponent field of the largest value -> the power that brings it to 2^13
+__device__ __forceinline__ int plane_power(uint32_t field) { return 140 - static_cast<int>(min(max(field, 13u), 254u)); }
+
+template <int HD>
+__global__ __launch_bounds__(256)
+void k_prompt_planes(PromptAttn p)
+{
+    constexpr int PIECES = PLANE_KEYS * HD / 8, PT = PIECES / 256;   // 8-value pieces of a thread, K or V
+    __shared__ uint32_t tops[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t tile = blockIdx.x, kvh = blockIdx.y;
+    // the tile's sequence
+    int32_t k0 = -1, nk = 0;
+    uint32_t local = 0, base = 0;
+    for (uint32_t i = 0; i < p.n_seqs && k0 < 0; i += WAVE) {
+        const PromptLane l = load_seq(p, i, lane);
+        const uint32_t n = plane_tiles(l), upto = base + wave_scan(n);
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            k0 = __builtin_amdgcn_readlane(l.ka, f);
+            nk = __builtin_amdgcn_readlane(l.kz, f) - k0;
+            local = tile - (readlane_u32(upto, f) - readlane_u32(n, f));
+        }
+        base = readlane_u32(upto, WAVE - 1);
+    }
+    if (k0 < 0) return;
+    const uint32_t keys = min(static_cast<uint32_t>(PLANE_KEYS), nk - local * PLANE_KEYS);
+    const uint64_t row0 = static_cast<uint64_t>(k0) + local * PLANE_KEYS;
+    float x[2][PT][8];
+    uint32_t top[2] = {0, 0};
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const uint32_t piece = threadIdx.x + 256 * i, row = piece / (HD / 8), c = piece % (HD / 8);
+            const float* src = static_cast<const float*>(v ? p.v : p.k) +
+                               (row0 + min(row, keys - 1)) * (v ? p.v_stride : p.k_stride) + kvh * HD + 8 * c;
+            load8(src, x[v][i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t bits = __float_as_uint(x[v][i][j]) & 0x7FFFFFFFu;
+                top[v] = max(top[v], bits < 0x7F800000u ? bits : 0u);
+            }
+        }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        top[v] = wave_max_u32(top[v]);
+        if (lane == 0) tops[v][wave] = top[v];
+    }
+    __syncthreads();
+    int power[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t t = max(max(tops[v][0], tops[v][1]), max(tops[v][2], tops[v][3]));
+        power[v] = plane_power(t >> 23);
+        if (v && t == 0) power[v] = NO_POWER;                   // (values of no size set no power for the sum)
+    }
+    if (threadIdx.x == 0) p.powers[static_cast<size_t>(kvh) * p.plane_tiles + tile] = make_int2(power[0], power[1]);
+    const size_t plane = static_cast<size_t>(p.k_rows) * p.num_kv_heads * HD;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const uint32_t piece = threadIdx.x + 256 * i, row = piece / (HD / 8), c = piece % (HD / 8);
+            if (row >= keys) continue;
+            float y[8], r[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j] = __builtin_amdgcn_ldexpf(x[v][i][j], power[v] == NO_POWER ? 0 : power[v]);
+                r[j] = y[j] - static_cast<float>(static_cast<_Float16>(y[j]));
+            }
+            const size_t at = 2 * v * plane + ((row0 + row) * p.num_kv_heads + kvh) * HD + 8 * c;
+            store8(reinterpret_cast<_Float16*>(p.planes) + at, y);
+            store8(reinterpret_cast<_Float16*>(p.planes) + at + plane, r);
+        }
 }
 
 template <int HD, typename T, int RW, int KG>
@@ -164,6 +281,9 @@ void k_attn_prompt(PromptAttn p)
     PromptSeq seq;
     if (!find_tile<ROWS>(p, tile, lane, seq)) return;
     const int32_t q0 = seq.q0, nq = seq.nq, k0 = seq.k0, nk = seq.nk;
+    // (sequences that share keys, around one whose offsets are wrong: more key tiles than the scratch holds)
+    if (S::F32 && static_cast<uint64_t>(seq.ktile) + static_cast<uint32_t>(nk + PLANE_KEYS - 1) / PLANE_KEYS > p.plane_tiles)
+        return;
     const int32_t before = nk - nq;                             // query i sees keys 0 .. i + before
     const uint32_t G = p.group, rows = static_cast<uint32_t>(nq) * G;
     // the longest tiles of a sequence first: what is left for the end of the launch is short
@@ -188,17 +308,50 @@ void k_attn_prompt(PromptAttn p)
     }
 
     // ---- the wave's query rows: B operands --------------------------------------
+    using M = std::conditional_t<S::F32, _Float16, T>;          // what the matrix cores take
     const uint32_t head = kvh * G + g;
     const T* qrow = static_cast<const T*>(p.q) + (static_cast<size_t>(q0) + qi) * p.q_stride + head * HD;
-    constexpr int QN = HD / (S::F32 ? 8 : 16);
-    uint4 qf[QN];
+    constexpr int QN = HD / 16;
+    uint4 qf[S::PLANES][QN];
+    float c2 = p.scale_log2;                                    // of the sums: scores in powers of two
+    int qpower = 0;
+    if constexpr (S::F32) {
+        // two f16 at a power of two that brings the row's largest value to 2^13 .. 2^14
+        float top = 0.f;
 #pragma unroll
-    for (int s = 0; s < QN; ++s) qf[s] = load_u4(reinterpret_cast<const uint8_t*>(qrow) + 32 * s + 16 * h);
+        for (int s = 0; s < QN; ++s) {
+            float x[8];
+            load8(qrow + 16 * s + 8 * h, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+        }
+        top = half_max(top);
+        const uint32_t field = (__float_as_uint(top) >> 23) & 0xFFu;
+        qpower = field == 255 ? 0 : plane_power(field);
+#pragma unroll
+        for (int s = 0; s < QN; ++s) {
+            float x[8];
+            load8(qrow + 16 * s + 8 * h, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_ldexpf(x[j], qpower);
+            split2(x[0], x[1], qf[0][s].x, qf[1][s].x);
+            split2(x[2], x[3], qf[0][s].y, qf[1][s].y);
+            split2(x[4], x[5], qf[0][s].z, qf[1][s].z);
+            split2(x[6], x[7], qf[0][s].w, qf[1][s].w);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < QN; ++s) qf[0][s] = load_u4(reinterpret_cast<const uint8_t*>(qrow) + 32 * s + 16 * h);
+    }
 
     // ---- direct loads: K and V tile t into buffer b ----------------------------
-    const uint64_t kb = p.k_stride * sizeof(T), vb = p.v_stride * sizeof(T);
-    const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + static_cast<uint64_t>(k0) * kb + kvh * RB;
-    const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + static_cast<uint64_t>(k0) * vb + kvh * RB;
+    const uint64_t kb = S::F32 ? nkv * RB : p.k_stride * sizeof(M), vb = S::F32 ? nkv * RB : p.v_stride * sizeof(M);
+    const uint64_t plane = S::F32 ? static_cast<uint64_t>(p.k_rows) * kb : 0;
+    const uint8_t* kbase = (S::F32 ? reinterpret_cast<const uint8_t*>(p.planes) : static_cast<const uint8_t*>(p.k)) +
+                           static_cast<uint64_t>(k0) * kb + kvh * RB;
+    const uint8_t* vbase = (S::F32 ? reinterpret_cast<const uint8_t*>(p.planes) + 2 * plane
+                                   : static_cast<const uint8_t*>(p.v)) +
+                           static_cast<uint64_t>(k0) * vb + kvh * RB;
     uint8_t* mine = smem + kg * S::LDS;
     const uint32_t lds0 = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
@@ -213,22 +366,26 @@ void k_attn_prompt(PromptAttn p)
     auto issue = [&](int32_t t, int b) {
         const uint8_t* kt = kbase + static_cast<uint64_t>(t) * KT * kb;
         const uint8_t* vt = vbase + static_cast<uint64_t>(t) * KT * vb;
-        const uint32_t to = lds0 + b * 2 * S::TILE + wv * NI * 1024;
+        const uint32_t to = lds0 + b * S::BUF + wv * NI * 1024;
         const int32_t last = nk - 1 - t * KT;
-        if (last >= KT - 1) {
 #pragma unroll
-            for (int u = 0; u < NI; ++u) {
-                load_to_lds(kt, koff[u], to + u * 1024);
-                load_to_lds(vt, voff[u], to + S::TILE + u * 1024);
-            }
-        } else {
-            // keys past the end: the last one again (masked)
+        for (int pl = 0; pl < S::PLANES; ++pl) {
+            const uint32_t kto = to + pl * S::TILE, vto = to + (S::PLANES + pl) * S::TILE;
+            if (last >= KT - 1) {
 #pragma unroll
-            for (int u = 0; u < NI; ++u) {
-                const int at = (wv * NI + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
-                const uint32_t src = static_cast<uint32_t>(min(row, last));
-                load_to_lds(kt, src * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row)), to + u * 1024);
-                load_to_lds(vt, src * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row)), to + S::TILE + u * 1024);
+                for (int u = 0; u < NI; ++u) {
+                    load_to_lds(kt + pl * plane, koff[u], kto + u * 1024);
+                    load_to_lds(vt + pl * plane, voff[u], vto + u * 1024);
+                }
+            } else {
+                // keys past the end: the last one again (masked)
+#pragma unroll
+                for (int u = 0; u < NI; ++u) {
+                    const int at = (wv * NI + u) * 1024 + lane * 16, row = at / RB, c = at % RB / 16;
+                    const uint32_t src = static_cast<uint32_t>(min(row, last));
+                    load_to_lds(kt + pl * plane, src * static_cast<uint32_t>(kb) + 16 * (c ^ S::kswz(row)), kto + u * 1024);
+                    load_to_lds(vt + pl * plane, src * static_cast<uint32_t>(vb) + 16 * (c ^ S::vswz(row)), vto + u * 1024);
+                }
             }
         }
     };
@@ -238,12 +395,13 @@ void k_attn_prompt(PromptAttn p)
     for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
-    float mx = -INFINITY, sum = 0.f;
-    const float c2 = p.scale_log2;
+    float mx = -INFINITY, sum = 0.f;                            // mx in powers of two
+    int vpower = NO_POWER;                                      // f32: acc holds the sum times 2^(15 + vpower)
+    const int2* powers = S::F32 ? p.powers + static_cast<size_t>(kvh) * p.plane_tiles + seq.ktile : nullptr;
 
-    auto tile_step = [&](int32_t t, int b) {
-        const uint8_t* kl = mine + b * 2 * S::TILE;
-        const uint8_t* vl = kl + S::TILE;
+    auto tile_step = [&](int32_t t, int b, int2 pw) {
+        const uint8_t* kl = mine + b * S::BUF;
+        const uint8_t* vl = kl + S::PLANES * S::TILE;
         // ---- S^T = K Q^T ----
         f32x16_t s[NSUB];
 #pragma unroll
@@ -254,15 +412,19 @@ void k_attn_prompt(PromptAttn p)
         for (int ks = 0; ks < QN; ++ks)
 #pragma unroll
             for (int u = 0; u < NSUB; ++u) {
-                const uint4 a = *reinterpret_cast<const uint4*>(kl + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col)));
+                const uint8_t* at = kl + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col));
+                const uint4 a = *reinterpret_cast<const uint4*>(at);
+                s[u] = mma16<M>(a, qf[0][ks], s[u]);
                 if constexpr (S::F32) {
-                    const f32x4v_t af = __builtin_bit_cast(f32x4v_t, a), bf = __builtin_bit_cast(f32x4v_t, qf[ks]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], s[u], 0, 0, 0);
-                } else {
-                    s[u] = mma16<T>(a, qf[ks], s[u]);
+                    s[u] = mma16<M>(a, qf[1][ks], s[u]);
+                    s[u] = mma16<M>(*reinterpret_cast<const uint4*>(at + S::TILE), qf[0][ks], s[u]);
                 }
             }
+        float sc = c2;
+        if constexpr (S::F32) {
+            // (never 0: a hidden key's -inf stays one)
+            sc = fmaxf(__builtin_amdgcn_ldexpf(c2, -qpower - pw.x), 0x1p-126f);
+        }
         // ---- the causal mask: keys t KT + 32 u + 8 (i / 4) + 4 h + i % 4 ----
         if (t * KT + KT - 1 > wave_first) {
             asm volatile("" : "+v"(s[0]));      // (a branch, not selects in every tile)
@@ -280,74 +442,81 @@ void k_attn_prompt(PromptAttn p)
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[u][i]);
-        mt = half_max(mt);
-        if (__ballot(mt > mx)) {
+        mt = half_max(mt) * sc;
+        if (__ballot(mt > mx) || (S::F32 && pw.y < vpower)) {
             const float mn = fmaxf(mx, mt);
-            const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f((mx - mn) * c2) : 0.f;
+            float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 0.f;
             sum *= f;
+            if constexpr (S::F32) {
+                const int vp = min(vpower, pw.y);
+                f = __builtin_amdgcn_ldexpf(f, vp - vpower);
+                vpower = vp;
+            }
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[d][i] *= f;
             mx = mn;
         }
-        const float mc = mx > -INFINITY ? mx * c2 : 0.f;        // (no key yet: every weight 0)
+        const float mc = mx > -INFINITY ? mx : 0.f;             // (no key yet: every weight 0)
+        const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, 15 + vpower - pw.y) : 1.f;
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c2, -mc));
-                if constexpr (S::F32) sum += s[u][i];
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], sc, -mc));
+                if constexpr (S::F32) {
+                    sum += s[u][i];
+                    s[u][i] *= pf;
+                }
             }
         // ---- O^T += V^T P^T ----
-        if constexpr (S::F32) {
+        // place c of a 16-lane group of a transposing read names row c / 4 and dims 4 (c % 4) .. of 16;
+        // the lane receives the rows' values of dim c
+        const int c = lane & 15, vrow = 4 * h + (c >> 2);
 #pragma unroll
-            for (int kk = 0; kk < KT / 8; ++kk)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const int c = 8 * d + col / 4;
-                        const float a = *reinterpret_cast<const float*>(vl + (8 * kk + 4 * h + j) * RB +
-                                                                        16 * (c ^ (h << 3)) + 4 * (col & 3));
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kk / 4][(kk % 4) * 4 + j], acc[d], 0, 0, 0);
-                    }
-        } else {
-            // lane (16-lane group g4 = 2 h + ..., place c) of a transposing read names row c / 4
-            // and dims 4 (c % 4) .. of 16; it receives the rows' values of dim c
-            const int c = lane & 15, vrow = 4 * h + (c >> 2);
-#pragma unroll
-            for (int ks = 0; ks < KT / 16; ++ks) {
-                uint4 pb;
-                const f32x16_t& sv = s[ks / 2];
-                const int o = (ks % 2) * 8;
-                pb.x = pack2<T>(sv[o + 0], sv[o + 1]);
-                pb.y = pack2<T>(sv[o + 2], sv[o + 3]);
-                pb.z = pack2<T>(sv[o + 4], sv[o + 5]);
-                pb.w = pack2<T>(sv[o + 6], sv[o + 7]);
+        for (int ks = 0; ks < KT / 16; ++ks) {
+            uint4 pb, pl;
+            const f32x16_t& sv = s[ks / 2];
+            const int o = (ks % 2) * 8;
+            if constexpr (S::F32) {
+                split2(sv[o + 0], sv[o + 1], pb.x, pl.x);
+                split2(sv[o + 2], sv[o + 3], pb.y, pl.y);
+                split2(sv[o + 4], sv[o + 5], pb.z, pl.z);
+                split2(sv[o + 6], sv[o + 7], pb.w, pl.w);
+            } else {
+                pb = make_uint4(pack2<T>(sv[o + 0], sv[o + 1]), pack2<T>(sv[o + 2], sv[o + 3]),
+                                pack2<T>(sv[o + 4], sv[o + 5]), pack2<T>(sv[o + 6], sv[o + 7]));
                 sum = add2<T>(pb.x, add2<T>(pb.y, add2<T>(pb.z, add2<T>(pb.w, sum))));
+            }
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const uint8_t* a = vl + (16 * ks + vrow) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
-                                       32 * ((lane >> 4) & 1) + 8 * (c & 3);
-                    typedef short s16x4_t __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
-                    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
-                    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 8 * RB));
-                    typedef short s16x8_t __attribute__((ext_vector_type(8)));
-                    const s16x8_t av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    acc[d] = mma16<T>(__builtin_bit_cast(uint4, av), pb, acc[d]);
+            for (int d = 0; d < ND; ++d) {
+                const uint8_t* at = vl + (16 * ks + vrow) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
+                                    32 * ((lane >> 4) & 1) + 8 * (c & 3);
+                const uint4 a = read_rows8(at, RB);
+                if constexpr (S::F32) {
+                    acc[d] = mma16<M>(a, pl, acc[d]);
+                    acc[d] = mma16<M>(read_rows8(at + S::TILE, RB), pb, acc[d]);
                 }
+                acc[d] = mma16<M>(a, pb, acc[d]);
             }
         }
     };
 
     // group kg takes tiles t0 + kg, t0 + kg + KG, ..
-    if (t0 + kg < t1) issue(t0 + kg, 0);
+    int2 pw = make_int2(0, 0);                                  // of the tile on its way
+    auto fetch = [&](int32_t t, int b) {
+        issue(t, b);
+        if constexpr (S::F32) pw = powers[t];
+    };
+    if (t0 + kg < t1) fetch(t0 + kg, 0);
     // The query loads end here: the compiler, which does not count the direct loads, would
     // otherwise wait for them at their use in the loop, and so for the next tile on its way.
 #pragma unroll
-    for (int s = 0; s < QN; ++s) asm volatile("" : "+v"(qf[s].x), "+v"(qf[s].y), "+v"(qf[s].z), "+v"(qf[s].w));
+    for (int s = 0; s < S::PLANES * QN; ++s) {
+        uint4& w = qf[s / QN][s % QN];
+        asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
+    }
     int b = 0;
     for (int32_t tt = t0; tt < t1; tt += KG, b ^= 1) {
         const int32_t t = tt + kg;
@@ -355,11 +524,18 @@ void k_attn_prompt(PromptAttn p)
         // the barrier so are every wave's
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + KG < t1) issue(t + KG, b ^ 1);
-        if (t * KT <= min(wave_last, t1 * KT - 1)) tile_step(t, b);
+        asm volatile("" : "+v"(pw.x), "+v"(pw.y)::"memory");    // (a load of the compiler's, as above)
+        const int2 at = pw;
+        if (t + KG < t1) fetch(t + KG, b ^ 1);
+        if (t * KT <= min(wave_last, t1 * KT - 1)) tile_step(t, b, at);
     }
     sum = half_sum(sum);
+    if constexpr (S::F32) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], -15 - vpower);
+    }
 
     // ---- the second key group's part joins the first's, lane by lane ---------------
     if constexpr (KG == 2) {
@@ -376,7 +552,7 @@ void k_attn_prompt(PromptAttn p)
         __syncthreads();
         if (kg == 1) return;
         const float m1 = other[ND * 16 * WAVE], mn = fmaxf(mx, m1), m0 = mn > -INFINITY ? mn : 0.f;
-        const float f0 = __builtin_amdgcn_exp2f((mx - m0) * c2), f1 = __builtin_amdgcn_exp2f((m1 - m0) * c2);
+        const float f0 = __builtin_amdgcn_exp2f(mx - m0), f1 = __builtin_amdgcn_exp2f(m1 - m0);
         sum = sum * f0 + other[(ND * 16 + 1) * WAVE] * f1;
         mx = mn;
 #pragma unroll
@@ -405,7 +581,7 @@ void k_attn_prompt(PromptAttn p)
         const size_t nrow = static_cast<size_t>(p.q_rows) * nkv * G;
         const size_t at = (row_out * nkv * G + head) * p.splits + blockIdx.y;
         if (h == 0) {
-            p.part[2 * at] = mx > -INFINITY ? mx * c2 : -INFINITY;
+            p.part[2 * at] = mx;
             p.part[2 * at + 1] = sum;
         }
         if (sum == 0.f) return;                                  // (the join reads no such part)
@@ -427,9 +603,14 @@ void k_prompt_join(PromptAttn p)
     const int lane = threadIdx.x & 63;
     const uint32_t heads = p.num_kv_heads * p.group;
     const uint32_t w = blockIdx.x * JOIN_WAVES + (threadIdx.x >> 6), row = w / heads;
-    if (row >= p.q_rows || static_cast<int32_t>(row) < p.q_offsets[0] ||
-        static_cast<int32_t>(row) >= p.q_offsets[p.n_seqs])
-        return;
+    if (row >= p.q_rows) return;
+    // (rows outside every sequence, or of one whose offsets are wrong, have no parts)
+    bool found = false;
+    for (uint32_t i = 0; i < p.n_seqs && !found; i += WAVE) {
+        const PromptLane l = load_seq(p, i, lane);
+        found = __ballot(l.ok && l.a <= static_cast<int32_t>(row) && static_cast<int32_t>(row) < l.z) != 0;
+    }
+    if (!found) return;
     const size_t nrow = static_cast<size_t>(p.q_rows) * heads, at = static_cast<size_t>(w) * p.splits;
     float o[HD / WAVE];
     join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(nrow, p.splits) + at * HD, p.splits, lane, o);
@@ -445,7 +626,8 @@ void k_prompt_join(PromptAttn p)
 //   4 x 1 beyond (two blocks a CU, nothing to merge): 4096 tokens 165 / 175 / 255, 64 sequences of 64 24 / 39 / 50.
 // Keys are split over blocks (each part eight tiles or more) until every CU has one: 64 tokens behind 8000 take
 // 101 in one part of 2 x 2 and 21 + 4 in eight; over long parts 4 x 2 is ahead again (256 tokens behind 4000:
-// 30 + 5 in four parts against 36 + 4 in two of 2 x 2).
+// 30 + 5 in four parts against 36 + 4 in two of 2 x 2).  f32 (tiles of 32) by the same rule: 512 tokens 22.9
+// against 28.2 (4 x 2), 23.7 + 4.3 (4 x 1 in two parts); 1024 49.5 against 61 + 8 (2 x 2), 51 + 8 (4 x 1).
 void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k)
 {
     constexpr uint64_t CUS = 256;
@@ -469,12 +651,34 @@ void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k
         a.splits = parts(b128);
     }
     a.tiles = static_cast<uint32_t>(rows / (32 * a.row_waves)) + a.n_seqs;
+    a.plane_tiles = f32 ? a.k_rows / PLANE_KEYS + std::min(a.n_seqs, a.k_rows) : 0;
 }
 
+// scratch: the f16 planes of f32 rows, their powers, then the parts of split keys
+static size_t plane_bytes(const PromptAttn& a, uint32_t head_dim)
+{
+    return (static_cast<size_t>(a.k_rows) * a.num_kv_heads * head_dim * 8 + 15) & ~size_t(15);
+}
+static size_t power_bytes(const PromptAttn& a)
+{
+    return (static_cast<size_t>(a.num_kv_heads) * a.plane_tiles * sizeof(int2) + 15) & ~size_t(15);
+}
 size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t head_dim)
 {
-    if (a.splits == 1) return 0;
-    return part_floats(static_cast<size_t>(a.q_rows) * a.num_kv_heads * a.group, a.splits, head_dim) * sizeof(float);
+    size_t n = 0;
+    if (a.plane_tiles) n += plane_bytes(a, head_dim) + power_bytes(a);
+    if (a.splits > 1) n += part_floats(static_cast<size_t>(a.q_rows) * a.num_kv_heads * a.group, a.splits, head_dim) * sizeof(float);
+    return n;
+}
+void prompt_scratch(PromptAttn& a, uint32_t head_dim, void* scratch)
+{
+    uint8_t* p = static_cast<uint8_t*>(scratch);
+    if (a.plane_tiles) {
+        a.planes = reinterpret_cast<uint16_t*>(p);
+        a.powers = reinterpret_cast<int2*>(p + plane_bytes(a, head_dim));
+        p += plane_bytes(a, head_dim) + power_bytes(a);
+    }
+    a.part = reinterpret_cast<float*>(p);
 }
 
 template <int HD, typename T, int RW, int KG>
@@ -501,6 +705,8 @@ hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t head_dim, uint3
         const uint32_t per = 8 % nkv == 0 ? 8 / nkv : 1;
         const dim3 grid((a.tiles + per - 1) / per * per * nkv, a.splits);
         hipError_t e;
+        if (a.plane_tiles)
+            launch_kernel(k_prompt_planes<HD>, dim3(a.plane_tiles, nkv), dim3(256), s, a);
         if (a.key_groups == 1) {
             e = launch_prompt<HD, T, 4, 1>(a, grid, s);
         } else if (a.row_waves == 2) {

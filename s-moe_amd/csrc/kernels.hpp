@@ -19,7 +19,7 @@ constexpr int SMOE_TOPK_MAX_K = 16;
 // marker packets around it).  Set only around eager launches by the profiling
 // path of the C ABI.
 struct DispatchTimer {
-    static constexpr int MAX = 2;             // dispatches of one launcher
+    static constexpr int MAX = 3;             // dispatches of one launcher
     struct Pair {
         hipEvent_t start = nullptr;
         hipEvent_t stop = nullptr;

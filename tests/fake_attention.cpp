@@ -46,6 +46,7 @@ size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t d)
 {
     return a.splits == 1 ? 0 : 4 * part_floats(size_t(a.q_rows) * a.num_kv_heads * a.group, a.splits, d);
 }
+void prompt_scratch(PromptAttn& a, uint32_t, void* p) { a.part = static_cast<float*>(p); }
 hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t, uint32_t, hipStream_t) { return booked(a.splits, a.part); }
 void kv4_plan(Kv4Attn& a, uint32_t, uint32_t max_len) { a.splits = std::max(1u, std::min(64u, max_len / 256)); }
 size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t d)
