@@ -97,9 +97,9 @@ struct Kv4Attn {
     uint64_t q_stride, out_stride;
     uint32_t n_seqs, group;     // group: query heads per KV head
     float scale_log2;
-    uint32_t splits;            // parts of a sequence's positions, joined by a second launch
-    uint32_t part_tiles;        // length of a part; more where a sequence would have more than `splits`
-    float* part;                // rows = sequences times heads (part_floats)
+    uint32_t units;             // parts of all sequences' positions for a KV head, joined by a second launch;
+                                // 0: each sequence whole
+    float* part;                // rows = units times heads (part_floats, one part a row)
     uint32_t* err;
 };
 void kv4_plan(Kv4Attn& a, uint32_t head_dim, uint32_t max_len);

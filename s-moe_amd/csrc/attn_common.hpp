@@ -84,6 +84,18 @@ __device__ __forceinline__ float half_sum(float v)
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// inclusive sum over the lanes up to this one
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
+{
+    v += dpp_u32<0x111>(0u, v);                 // row_shr 1, 2, 4, 8
+    v += dpp_u32<0x112>(0u, v);
+    v += dpp_u32<0x114>(0u, v);
+    v += dpp_u32<0x118>(0u, v);
+    v += dpp_u32<DPP_ROW_BCAST15, 0xA>(0u, v);
+    v += dpp_u32<DPP_ROW_BCAST31, 0xC>(0u, v);
+    return v;
+}
+
 // any lane of a block that finds a bad index says so
 __device__ __forceinline__ void flag_range(uint32_t* err)
 {
@@ -92,36 +104,42 @@ __device__ __forceinline__ void flag_range(uint32_t* err)
 
 // The partial results of one output row, in `splits` parts: out = sum_s f_s o_s /
 // sum_s f_s l_s with f_s = 2^(m_s - max m).  Parts without a key (l = 0) hold no o_s.
-// One wave per output row: reads its parts and leaves the joined row in o, lane l's
-// dims at l * HD / 64.  All the parts' loads of a pass of eight are in flight at once.
+// One wave per output row: reads its parts, `step` parts apart, and leaves the joined row
+// in o, lane l's dims at l * HD / 64.  A pass's loads, of 16 parts, are in flight at once.
 template <int HD>
-__device__ __forceinline__ void join_parts(const float* ml, const float* acc, uint32_t splits, int lane, float (&o)[HD / WAVE])
+__device__ __forceinline__ void join_parts(const float* ml, const float* acc, uint32_t splits, uint32_t step, int lane,
+                                           float (&o)[HD / WAVE])
 {
     constexpr int DV = HD / WAVE;
+    constexpr uint32_t PASS = 16;
     const bool live = static_cast<uint32_t>(lane) < splits;
-    const float m = live ? ml[2 * lane] : -INFINITY, l = live ? ml[2 * lane + 1] : 0.f;
+    const size_t mine = static_cast<size_t>(lane) * step;
+    const float m = live ? ml[2 * mine] : -INFINITY, l = live ? ml[2 * mine + 1] : 0.f;
     const bool used = l != 0.f;                          // (a NaN sum is used)
     const float top = wave_max(used ? m : -INFINITY);
     const float f = used ? exp2f(m - (top > -INFINITY ? top : 0.f)) : 0.f;
     const float sum = wave_sum(used ? f * l : 0.f);
-    const uint64_t parts = __ballot(used);
+    const uint32_t keep = used ? 0xFFFFFFFFu : 0u;
 #pragma unroll
     for (int j = 0; j < DV; ++j) o[j] = 0.f;
-    for (uint32_t s0 = 0; s0 < splits; s0 += 8) {
-        float a[8][DV], t[DV];
+    for (uint32_t s0 = 0; s0 < splits; s0 += PASS) {
+        float a[PASS][DV], t[DV];
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
-            const bool on = s0 + u < splits && ((parts >> (s0 + u)) & 1);
+        for (uint32_t u = 0; u < PASS; ++u) {
+            // (loaded in any case, the last part's again past the end: a branch would keep the loads apart)
+            const float* row = acc + static_cast<size_t>(min(s0 + u, splits - 1)) * step * HD + lane * DV;
 #pragma unroll
-            for (int j = 0; j < DV; ++j) a[u][j] = on ? acc[static_cast<size_t>(s0 + u) * HD + lane * DV + j] : 0.f;
+            for (int j = 0; j < DV; ++j) a[u][j] = row[j];
         }
 #pragma unroll
         for (int j = 0; j < DV; ++j) t[j] = 0.f;
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
+        for (uint32_t u = 0; u < PASS; ++u) {
+            // (a part without a key may hold anything, so its bits are cleared: again no branch)
             const float fs = readlane_f32(f, (s0 + u) & 63);
+            const uint32_t bits = readlane_u32(keep, (s0 + u) & 63);
 #pragma unroll
-            for (int j = 0; j < DV; ++j) t[j] = fmaf(fs, a[u][j], t[j]);
+            for (int j = 0; j < DV; ++j) t[j] = fmaf(fs, __uint_as_float(__float_as_uint(a[u][j]) & bits), t[j]);
         }
 #pragma unroll
         for (int j = 0; j < DV; ++j) o[j] += t[j];

@@ -15,9 +15,10 @@
 //     Scores come out transposed, S^T = K Q^T: lane (m = l & 15, q = l >> 4) has the
 //     scores of head m at positions 4 q + i (+ 16), which are the B operand of the
 //     weighted sum O^T = V^T P^T as they stand.  P is multiplied by the V scale of its
-//     position and group first and put in f16 (bf16 results: once, its 11 bits against
-//     the result's 8; else twice like q), at a power of two that the largest scale of the
-//     group so far sets: the mins' part, sum p m_g, is one fp32 sum a group.
+//     position and group first and put in f16 twice like q, at a power of two that the
+//     largest scale of the group so far sets (once would save 5 % of a bf16 call, but code
+//     times scale and min may cancel, and then its 11 bits are not enough for a bf16 result):
+//     the mins' part, sum p m_g, is one fp32 sum a group.
 //     A tile's bytes come by direct loads into the wave's own two LDS buffers, one tile
 //     ahead, with no register held meanwhile: 128 registers leave four waves a SIMD, whose
 //     loads in flight and whose arithmetic cover each other.  K operands are 8-byte reads
@@ -25,7 +26,11 @@
 //     of two dims); 16-byte pieces of a row are exchanged so that neither meets a bank
 //     twice.  The 16 lanes that share a position would unpack the same scales and mins, so
 //     each pair is put into floats by one lane and passed on through LDS.
-//   k_kv4_join   the parts of each (sequence, head) joined.
+//     Bound: the cache's bytes where there are many (head_dim 128, 4 KV heads: 48 sequences of
+//     8192, bf16, 226 MB in 53 us, 4.3 TB/s; 16 of 32768, 64 query heads, f32, 302 MB in
+//     70 us, 4.3 TB/s, of which the loads alone take 58; a large copy reaches 5.1 TB/s), else
+//     the launch and one chain of length, tile and query loads: one sequence of 777, 7 us.
+//   k_kv4_join   the parts of each (sequence, head) joined (4 us, 5 with 64 parts a row).
 #include <algorithm>
 
 #include "attn_common.hpp"
@@ -120,6 +125,61 @@ struct Kv4Shape {
     __host__ __device__ static constexpr int swz(int r) { return r / (256 / RB) & (PIECES - 1); }
 };
 
+// ---------------------------------------------------------------------------
+// Which positions a block takes.  The sequences' tiles are cut into p.units parts or fewer
+// of the same length, as near as may be, so that sequences of different lengths give every
+// block the same work (32 sequences of up to 8192: 24 us against 26 with the longest one's
+// parts for all): the shortest length at which the parts of all sequences are few enough.
+// Every wave works it out from the lengths, 64 sequences a pass; for more than 64 it takes
+// the length that is enough at any rate.
+// ---------------------------------------------------------------------------
+struct Kv4Seq {                                 // a lane's sequence
+    int32_t slot;
+    uint32_t n, tiles;                          // positions (0: none, or an index out of range)
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, uint32_t b, bool flag)
+{
+    const uint32_t at = min(b, p.n_seqs - 1);
+    Kv4Seq s{p.slots ? p.slots[at] : static_cast<int32_t>(at), static_cast<uint32_t>(p.lens[at]), 0};
+    if (static_cast<uint32_t>(s.slot) >= p.c.n_slots || s.n > p.c.capacity) {   // (or below zero)
+        if (flag && b < p.n_seqs) flag_range(p.err);
+        s.slot = 0;
+        s.n = 0;
+    }
+    if (b >= p.n_seqs) s.n = 0;
+    s.tiles = (s.n + KA_TILE - 1) / KA_TILE;
+    return s;
+}
+// ceil(tiles / part), for tiles below 2^20: the product may fall short of a whole quotient by
+// its rounding, never reach past the next
+__device__ __forceinline__ uint32_t kv4_parts(uint32_t tiles, uint32_t part)
+{
+    const uint32_t c = static_cast<uint32_t>(static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(part)));
+    return c * part < tiles ? c + 1 : c;
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) { return readlane_u32(wave_scan(v), WAVE - 1); }
+// tiles of a part; s: the lane's sequence of the first 64; flag: says so if one of the others is out of range
+__device__ __forceinline__ uint32_t kv4_part_tiles(const Kv4Attn& p, int lane, const Kv4Seq& s, bool flag)
+{
+    uint32_t total = wave_total(s.tiles), top = wave_max_u32(s.tiles);
+    for (uint32_t i = WAVE; i < p.n_seqs; i += WAVE) {
+        const uint32_t t = kv4_seq(p, i + lane, flag).tiles;
+        total += wave_total(t);
+        top = max(top, wave_max_u32(t));
+    }
+    // (a tile a wave, and no more parts than the join takes)
+    uint32_t lo = max(max(static_cast<uint32_t>(KA_WAVES), (top + JOIN_MAX - 1) / JOIN_MAX), (total + p.units - 1) / p.units);
+    // enough at any rate: total / part + one a sequence
+    uint32_t hi = max(lo, p.units > p.n_seqs ? (total + p.units - p.n_seqs - 1) / (p.units - p.n_seqs) : top);
+    if (p.n_seqs > WAVE) return hi;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (wave_total(kv4_parts(s.tiles, mid)) <= p.units) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
 template <int HD, typename T>
 __global__ __launch_bounds__(KA_THREADS, (Kv4Shape<HD>::WAVES_PER_SIMD))
 void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
@@ -127,7 +187,6 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
     using S = Kv4Shape<HD>;
     constexpr int NG = S::NG, RB = S::RB, RS = S::RS;
     constexpr bool Q2 = sizeof(T) == 4;         // q as two f16
-    constexpr bool P2 = !__is_same(T, __bf16);  // P as two f16
     extern __shared__ __align__(16) float buf[];    // the waves' tiles; before and after, rows of heads
     __shared__ float qsum[KA_HEADS * NG], mw[KA_WAVES * KA_HEADS], lw[KA_WAVES * KA_HEADS];
 
@@ -135,34 +194,42 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
     const int m16 = lane & 15, q = lane >> 4;
     const uint32_t G = p.group, nkv = p.c.num_kv_heads;
     const uint32_t sub = blockIdx.x % n_sub, kvh = blockIdx.x / n_sub % nkv;
-    // the sequences one further with every part: else those that share a remainder of the XCDs'
-    // number would all run on one XCD (32 of 52 to 8192 positions: 31 us against 26)
-    const uint32_t seq = (blockIdx.x / n_sub / nkv + blockIdx.y) % p.n_seqs;
+    const uint32_t unit = blockIdx.x / n_sub / nkv;
     const uint32_t hbase = kvh * G + sub * KA_HEADS;            // first query head of the block
     const uint32_t ng = min(static_cast<uint32_t>(KA_HEADS), G - sub * KA_HEADS);
     const uint32_t heads = nkv * G;
-    const size_t nrow = static_cast<size_t>(p.n_seqs) * heads;
 
     // ---- the block's positions ------------------------------------------------
-    const int32_t slot = __builtin_amdgcn_readfirstlane(p.slots ? p.slots[seq] : static_cast<int32_t>(seq));
-    const int32_t len = __builtin_amdgcn_readfirstlane(p.lens[seq]);
-    uint32_t n = static_cast<uint32_t>(len);
-    if (static_cast<uint32_t>(slot) >= p.c.n_slots || len < 0 || n > p.c.capacity) {
-        if (threadIdx.x == 0) flag_range(p.err);
-        n = 0;                                                  // (a row of zeros)
-    }
-    // parts of `part` tiles, so that sequences of different lengths give blocks of the same work
-    const uint32_t tiles = (n + KA_TILE - 1) / KA_TILE, part = max(p.part_tiles, (tiles + p.splits - 1) / p.splits);
-    const uint32_t t0 = min(tiles, blockIdx.y * part), t1 = min(tiles, t0 + part);
-    if (t0 >= t1 && p.splits > 1) {
-        if (threadIdx.x < ng) {
-            const size_t at = (static_cast<size_t>(seq) * heads + hbase + threadIdx.x) * p.splits + blockIdx.y;
-            p.part[2 * at] = -INFINITY;
-            p.part[2 * at + 1] = 0.f;
+    uint32_t seq = unit, n, t0 = 0, t1, parts = 1;
+    int32_t slot;
+    if (p.units) {
+        Kv4Seq s = kv4_seq(p, lane, blockIdx.x == 0);
+        const uint32_t part = kv4_part_tiles(p, lane, s, blockIdx.x == 0);
+        for (uint32_t i = 0, base = 0;;) {
+            const uint32_t c = kv4_parts(s.tiles, part), upto = base + wave_scan(c);
+            if (const uint64_t past = __ballot(upto > unit)) {
+                const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                seq = i + f;
+                n = readlane_u32(s.n, f);
+                slot = __builtin_amdgcn_readlane(s.slot, f);
+                parts = readlane_u32(c, f);
+                const uint32_t tiles = readlane_u32(s.tiles, f), len = kv4_parts(tiles, parts);
+                t0 = (unit - (readlane_u32(upto, f) - parts)) * len;
+                t1 = min(tiles, t0 + len);
+                break;
+            }
+            base = readlane_u32(upto, WAVE - 1);
+            i += WAVE;
+            if (i >= p.n_seqs) return;                          // (fewer parts than units)
+            s = kv4_seq(p, i + lane, false);
         }
-        return;
+    } else {
+        const Kv4Seq s = kv4_seq(p, seq, threadIdx.x == 0);
+        n = __builtin_amdgcn_readfirstlane(s.n);
+        slot = __builtin_amdgcn_readfirstlane(s.slot);
+        t1 = __builtin_amdgcn_readfirstlane(s.tiles);
     }
-    const size_t line0 = (static_cast<size_t>(n ? slot : 0) * nkv + kvh) * p.c.capacity;
+    const size_t line0 = (static_cast<size_t>(slot) * nkv + kvh) * p.c.capacity;
     const uint8_t* kc = p.c.codes[0] + line0 * RB;
     const uint8_t* vc = p.c.codes[1] + line0 * RB;
     const uint8_t* kpar = reinterpret_cast<const uint8_t*>(p.c.params[0]) + line0 * (4 * NG);
@@ -377,15 +444,10 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
                 }
             }
             // in the order of codes8's places
-            if constexpr (P2) {
-                split2(y[code_at(0)], y[code_at(1)], hi.x, lo.x);
-                split2(y[code_at(2)], y[code_at(3)], hi.y, lo.y);
-                split2(y[code_at(4)], y[code_at(5)], hi.z, lo.z);
-                split2(y[code_at(6)], y[code_at(7)], hi.w, lo.w);
-            } else {
-                hi = make_uint4(pack2<_Float16>(y[code_at(0)], y[code_at(1)]), pack2<_Float16>(y[code_at(2)], y[code_at(3)]),
-                                pack2<_Float16>(y[code_at(4)], y[code_at(5)]), pack2<_Float16>(y[code_at(6)], y[code_at(7)]));
-            }
+            split2(y[code_at(0)], y[code_at(1)], hi.x, lo.x);
+            split2(y[code_at(2)], y[code_at(3)], hi.y, lo.y);
+            split2(y[code_at(4)], y[code_at(5)], hi.z, lo.z);
+            split2(y[code_at(6)], y[code_at(7)], hi.w, lo.w);
             const f16x8_t ph = __builtin_bit_cast(f16x8_t, hi), pl = __builtin_bit_cast(f16x8_t, lo);
 #pragma unroll
             for (int e2 = 0; e2 < 2; ++e2) {
@@ -396,7 +458,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
                 for (int d2 = 0; d2 < 2; ++d2) {
                     const f16x8_t cv = codes8(static_cast<uint32_t>(w[d2]), even, odd);
                     f32x4v_t& o = acc[g][2 * e2 + d2];
-                    if constexpr (P2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, pl, o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, pl, o, 0, 0, 0);
                     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(cv, ph, o, 0, 0, 0);
                 }
             }
@@ -441,11 +503,11 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
             L = fmaf(f, lw[w * KA_HEADS + g], L);
             A = fmaf(f, buf[(w * KA_HEADS + g) * RS + d], A);
         }
-        if (p.splits == 1) {
+        if (parts == 1) {
             static_cast<T*>(p.out)[seq * p.out_stride + head * HD + d] = static_cast<T>(L == 0.f ? 0.f : A * (1.0f / L));
         } else {
-            const size_t at = (static_cast<size_t>(seq) * heads + head) * p.splits + blockIdx.y;
-            p.part[part_acc_at(nrow, p.splits) + at * HD + d] = A;
+            const size_t at = static_cast<size_t>(unit) * heads + head;
+            p.part[part_acc_at(static_cast<size_t>(p.units) * heads, 1) + at * HD + d] = A;
             if (d == 0) {
                 p.part[2 * at] = M;
                 p.part[2 * at + 1] = L;
@@ -461,32 +523,44 @@ void k_kv4_join(Kv4Attn p)
 {
     const int lane = threadIdx.x & 63;
     const uint32_t heads = p.c.num_kv_heads * p.group;
-    const uint32_t w = blockIdx.x * KA_WAVES + (threadIdx.x >> 6), seq = w / heads;
+    const uint32_t w = blockIdx.x * KA_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seq = w / heads;
     if (seq >= p.n_seqs) return;
-    const size_t nrow = static_cast<size_t>(p.n_seqs) * heads, at = static_cast<size_t>(w) * p.splits;
+    // the sequence's parts, as its blocks found them
+    Kv4Seq s = kv4_seq(p, lane, false);
+    const uint32_t part = kv4_part_tiles(p, lane, s, false);
+    uint32_t base = 0, c = kv4_parts(s.tiles, part), i = 0;
+    for (; i + WAVE <= seq; i += WAVE) {
+        base += wave_total(c);
+        s = kv4_seq(p, i + WAVE + lane, false);
+        c = kv4_parts(s.tiles, part);
+    }
+    const uint32_t upto = base + wave_scan(c);
+    const uint32_t parts = readlane_u32(c, seq - i), first = readlane_u32(upto, seq - i) - parts;
+    if (parts == 1) return;                                     // (its block wrote the row)
+    const size_t at = static_cast<size_t>(first) * heads + w % heads;
     float o[HD / WAVE];
-    join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(nrow, p.splits) + at * HD, p.splits, lane, o);
+    join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(static_cast<size_t>(p.units) * heads, 1) + at * HD, parts, heads,
+                   lane, o);
     store_row<HD>(static_cast<T*>(p.out) + seq * p.out_stride + (w % heads) * HD, o, lane);
 }
 
 void kv4_plan(Kv4Attn& a, uint32_t head_dim, uint32_t max_len)
 {
     const uint32_t n_sub = (a.group + KA_HEADS - 1) / KA_HEADS;
-    const uint64_t blocks = static_cast<uint64_t>(a.n_seqs) * a.c.num_kv_heads * n_sub;
-    const uint32_t tiles = max_len / KA_TILE + (max_len % KA_TILE != 0);
-    // As many blocks as are resident at once (256 CUs of four, or two at head_dim 256), each with a tile a
+    const uint32_t quads = max_len / (KA_WAVES * KA_TILE) + (max_len % (KA_WAVES * KA_TILE) != 0);
+    // As many parts as blocks are resident at once (256 CUs of four, or two at head_dim 256), each with a tile a
     // wave or more: 16 sequences of 32768 over 4 KV heads 72.8 us in 16 parts (1024 blocks), 78.0 in 8, 74.8
-    // in 12, 76.2 in 24; one of 777 over 4 KV heads 6.9 us in 7 parts, 8.5 in 6, 15.5 in one.
-    const uint32_t resident = head_dim == 256 ? 512 : 1024;
-    const uint64_t most = std::min<uint64_t>(JOIN_MAX, resident / std::max<uint64_t>(1, blocks));
-    a.splits = std::max<uint32_t>(1, std::min<uint32_t>(static_cast<uint32_t>(most), (tiles + KA_WAVES - 1) / KA_WAVES));
-    a.part_tiles = (tiles + a.splits - 1) / a.splits;
+    // in 12, 76.2 in 24; one of 777 over 4 KV heads 6.9 us in 7 parts, 8.5 in 6, 15.5 in one.  Sequences whole
+    // where they fill half of that, or no sequence has a second part.
+    const uint32_t most = (head_dim == 256 ? 512 : 1024) / (a.c.num_kv_heads * n_sub);
+    a.units = static_cast<uint32_t>(std::min<uint64_t>(most, static_cast<uint64_t>(a.n_seqs) * quads));
+    if (a.units < 2 * static_cast<uint64_t>(a.n_seqs)) a.units = 0;
 }
 
 size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t head_dim)
 {
-    if (a.splits == 1) return 0;
-    return part_floats(static_cast<size_t>(a.n_seqs) * a.c.num_kv_heads * a.group, a.splits, head_dim) * sizeof(float);
+    if (a.units == 0) return 0;
+    return part_floats(static_cast<size_t>(a.units) * a.c.num_kv_heads * a.group, 1, head_dim) * sizeof(float);
 }
 
 hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t head_dim, uint32_t type, hipStream_t s)
@@ -501,9 +575,9 @@ hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t head_dim, uint32_t ty
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
             if (e != hipSuccess) return e;
         }
-        launch_kernel_lds(k_attn_kv4<HD, T>, dim3(a.n_seqs * a.c.num_kv_heads * n_sub, a.splits), dim3(KA_THREADS),
-                          lds, s, a, n_sub);
-        if (a.splits > 1)
+        launch_kernel_lds(k_attn_kv4<HD, T>, dim3((a.units ? a.units : a.n_seqs) * a.c.num_kv_heads * n_sub),
+                          dim3(KA_THREADS), lds, s, a, n_sub);
+        if (a.units)
             launch_kernel(k_kv4_join<HD, T>, dim3((a.n_seqs * heads + KA_WAVES - 1) / KA_WAVES), dim3(KA_THREADS), s, a);
         return hipGetLastError();
     });

@@ -101,18 +101,6 @@ __device__ __forceinline__ float add2(uint32_t w, float c)
     }
 }
 
-// inclusive sum over the lanes up to this one
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
-{
-    v += dpp_u32<0x111>(0u, v);                 // row_shr 1, 2, 4, 8
-    v += dpp_u32<0x112>(0u, v);
-    v += dpp_u32<0x114>(0u, v);
-    v += dpp_u32<0x118>(0u, v);
-    v += dpp_u32<DPP_ROW_BCAST15, 0xA>(0u, v);
-    v += dpp_u32<DPP_ROW_BCAST31, 0xC>(0u, v);
-    return v;
-}
-
 // The sequence of row tile `tile` (ROWS rows each), by the whole wave; false past the last one.
 // Sequences whose offsets point outside their rows have no tiles.
 struct PromptSeq {
@@ -613,7 +601,7 @@ void k_prompt_join(PromptAttn p)
     if (!found) return;
     const size_t nrow = static_cast<size_t>(p.q_rows) * heads, at = static_cast<size_t>(w) * p.splits;
     float o[HD / WAVE];
-    join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(nrow, p.splits) + at * HD, p.splits, lane, o);
+    join_parts<HD>(p.part + 2 * at, p.part + part_acc_at(nrow, p.splits) + at * HD, p.splits, 1, lane, o);
     store_row<HD>(static_cast<T*>(p.out) + row * p.out_stride + (w % heads) * HD, o, lane);
 }
 

@@ -48,10 +48,10 @@ size_t prompt_scratch_bytes(const PromptAttn& a, uint32_t d)
 }
 void prompt_scratch(PromptAttn& a, uint32_t, void* p) { a.part = static_cast<float*>(p); }
 hipError_t launch_attention_prompt(const PromptAttn& a, uint32_t, uint32_t, hipStream_t) { return booked(a.splits, a.part); }
-void kv4_plan(Kv4Attn& a, uint32_t, uint32_t max_len) { a.splits = std::max(1u, std::min(64u, max_len / 256)); }
+void kv4_plan(Kv4Attn& a, uint32_t, uint32_t max_len) { a.units = max_len < 512 ? 0 : a.n_seqs * std::min(64u, max_len / 256); }
 size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t d)
 {
-    return a.splits == 1 ? 0 : 4 * part_floats(size_t(a.n_seqs) * a.c.num_kv_heads * a.group, a.splits, d);
+    return a.units == 0 ? 0 : 4 * part_floats(size_t(a.units) * a.c.num_kv_heads * a.group, 1, d);
 }
-hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t, uint32_t, hipStream_t) { return booked(a.splits, a.part); }
+hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t, uint32_t, hipStream_t) { return booked(a.units ? 2 : 1, a.part); }
 }  // namespace smoe
