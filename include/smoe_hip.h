@@ -441,6 +441,9 @@ int smoe_hip_attention_layer(SmoeMetalCtx* ctx, const SmoeAttnLayerArgs* args);
  *   - packed sequences: sequence b has rows offsets[b] .. offsets[b+1]-1;
  *     offsets ascend, and rows outside every sequence are neither read nor
  *     written;
+ *   - sizes that a launch cannot hold are refused (SMOE_ERR_SHAPE): 2^26 rows of
+ *     the row calls, 2^29 query rows times heads or 2^21 sequences times KV heads
+ *     of prompts (f32: 2^28 key rows), 2^24 sequences times heads over the cache;
  *   - offsets, slots, positions and lengths live on the device.  One that
  *     points outside its buffer is never followed: the call skips or zeroes
  *     what it concerns and the next smoe_hip_synchronize returns SMOE_ERR_ARG;
@@ -624,8 +627,9 @@ int smoe_hip_moe_decode_static(const SmoeMoeShape* shape, const SmoeMoeLayer* la
  * When enabled, every kernel the context launches outside graph capture is
  * bracketed by HIP events on the stream it runs on; profile_read returns the
  * launch count and summed event time of one kernel kind.  A kind that takes two
- * dispatches a call (PERMUTE over several segments, the ATTENTION kinds over
- * several parts of the keys) counts one launch with the time of both. */
+ * or three dispatches a call (PERMUTE over several segments, the ATTENTION kinds
+ * over several parts of the keys or of f32 prompts) counts one launch with the
+ * time of all. */
 #define SMOE_KERNEL_MOE_UP        0   /* RMSNorm + router + top-k + gate/up GEMV + SiLU */
 #define SMOE_KERNEL_GATE_UP       1   /* gate/up GEMV + SiLU (reference surface)        */
 #define SMOE_KERNEL_MOE_DOWN      2   /* down GEMV + weighted combine + residual        */

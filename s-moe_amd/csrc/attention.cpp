@@ -10,6 +10,8 @@
 namespace {
 
 constexpr uint64_t kMostRows = 1ull << 31;      // rows times heads of a call
+// a launch has less than 2^32 threads: of the row kernels a wave a row or less, or 8192 in all
+constexpr uint64_t kMostRowWaves = (1ull << 26) - 4;
 constexpr uint64_t kMostStride = 1ull << 22;    // elements between rows
 constexpr uint32_t kMostHeads = 1024;
 constexpr uint32_t kMostPositions = 1u << 24;   // of a cache slot
@@ -103,7 +105,8 @@ int check_kv4_rows(SmoeMetalCtx* ctx, const SmoeKv4Cache* c, const SmoeKv4RowsAr
     for (const auto& r : {std::pair<const void*, uint64_t>(a->k, a->k_stride), {a->v, a->v_stride}})
         if (const char* why = bad_rows(r.first, r.second, cols, a->type)) return refuse(ctx, SMOE_ERR_SHAPE, why);
     // (a row's groups of 64 are dealt to waves in 32 bits)
-    if (uint64_t(a->n_rows) * 2 * c->num_kv_heads * (c->head_dim / 64) >= kMostRows || a->n_seqs >= kMostRows)
+    if (uint64_t(a->n_rows) * 2 * c->num_kv_heads * (c->head_dim / 64) >= kMostRows || a->n_rows > kMostRowWaves ||
+        a->n_seqs >= kMostRows)
         return refuse(ctx, SMOE_ERR_SHAPE, "too many rows");
     return SMOE_OK;
 }
@@ -157,7 +160,7 @@ extern "C" int smoe_hip_qk_norm_rope(SmoeMetalCtx* ctx, const SmoeQkRowsArgs* a)
         if (why) return refuse(ctx, SMOE_ERR_SHAPE, why);
         r.num_kv_heads = a->num_kv_heads;
     }
-    if (uint64_t(a->n_rows) * (r.num_heads + r.num_kv_heads) >= kMostRows)
+    if (uint64_t(a->n_rows) * (r.num_heads + r.num_kv_heads) >= kMostRows || a->n_rows > kMostRowWaves)
         return refuse(ctx, SMOE_ERR_SHAPE, "too many rows");
     if (a->n_rows == 0) return SMOE_OK;
     const smoe::ContextView v = smoe::context_view(ctx);
@@ -202,8 +205,9 @@ extern "C" int smoe_hip_attention_prompt(SmoeMetalCtx* ctx, const SmoePromptAttn
     if (a->k_rows)
         for (const auto& r : {std::pair<const void*, uint64_t>(a->k, a->k_stride), {a->v, a->v_stride}})
             if (const char* why = bad_rows(r.first, r.second, kc, a->type)) return refuse(ctx, SMOE_ERR_SHAPE, why);
-    if (uint64_t(a->q_rows) * a->num_heads >= kMostRows || a->k_rows >= kMostRows ||
-        (uint64_t(a->n_seqs) + 8) * a->num_kv_heads >= kMostRows / 2)
+    // (threads of a launch: 4 a row and head and 512 a sequence and KV head, or 8 a f32 key row and 256 a sequence)
+    if (uint64_t(a->q_rows) * a->num_heads >= kMostRows / 4 || (uint64_t(a->n_seqs) + 8) * a->num_kv_heads >= 1u << 21 ||
+        a->k_rows >= (a->type == SMOE_TYPE_F32 ? kMostRows / 8 : kMostRows))
         return refuse(ctx, SMOE_ERR_SHAPE, "too many rows or sequences");
     if (a->q_rows == 0) return SMOE_OK;
     const smoe::ContextView v = smoe::context_view(ctx);
@@ -280,7 +284,8 @@ extern "C" int smoe_hip_attention_kv4(SmoeMetalCtx* ctx, const SmoeKv4Cache* c, 
     const uint64_t cols = uint64_t(a->num_heads) * c->head_dim;
     for (const auto& r : {std::pair<const void*, uint64_t>(a->q, a->q_stride), {a->out, a->out_stride}})
         if (const char* why = bad_rows(r.first, r.second, cols, a->type)) return refuse(ctx, SMOE_ERR_SHAPE, why);
-    if (uint64_t(a->n_seqs) * a->num_heads >= kMostRows) return refuse(ctx, SMOE_ERR_SHAPE, "too many sequences");
+    // (256 threads a sequence and KV head, or 16 heads of it)
+    if (uint64_t(a->n_seqs) * a->num_heads >= 1u << 24) return refuse(ctx, SMOE_ERR_SHAPE, "too many sequences");
     const smoe::ContextView v = smoe::context_view(ctx);
     const OnDevice on(v.device);
     if (!on.ok()) return refuse(ctx, SMOE_ERR_HIP, "hipSetDevice failed");

@@ -10,8 +10,9 @@
 //     (two codes a word by one and-or with the bits of 1024 or 64 and one packed
 //     subtraction), the scales and mins are applied to the fp32 sums of a group:
 //       q . k_j = sum_g s_g (sum c q) + m_g (sum_g q)
-//     The query goes in as f16, at a power of two a head that keeps it in range: exact
-//     for 16-bit types; f32 twice, the value and what its rounding left (22 bits).
+//     The query goes in as f16, at a power of two that brings the head's largest value to
+//     8 .. 16: 16-bit types once (exact, but for values under 2^-17 of that one, which keep
+//     2^-28 of it), f32 twice, the value and what its rounding left (22 bits).
 //     Scores come out transposed, S^T = K Q^T: lane (m = l & 15, q = l >> 4) has the
 //     scores of head m at positions 4 q + i (+ 16), which are the B operand of the
 //     weighted sum O^T = V^T P^T as they stand.  P is multiplied by the V scale of its

@@ -13,6 +13,7 @@
 #include <atomic>
 #include <cstdio>
 #include <cstring>
+#include <new>
 #include <vector>
 
 #include "context.hpp"
@@ -510,6 +511,11 @@ int context_attention_scratch(SmoeMetalCtx* ctx, size_t bytes, float** p)
         // (twice what a captured graph keeps alive, so that what stays behind is bounded)
         const size_t want = b.captured ? std::max(n, 2 * b.n) : n;
         float* grown = nullptr;
+        try {
+            ctx->attn_rows_old.reserve(ctx->attn_rows_old.size() + 1);
+        } catch (const std::bad_alloc&) {
+            return context_refuse(ctx, SMOE_ERR_HIP, "out of host memory");
+        }
         if (!dalloc(ctx, &grown, want)) return SMOE_ERR_HIP;
         if (b.p && b.captured) {
             ctx->attn_rows_old.push_back(b.p);

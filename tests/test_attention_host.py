@@ -158,6 +158,21 @@ def test_cache_rows(lib, more, rc):
     assert lib.call("kv4_read", cache(), rows(**more)) == rc
 
 
+def test_the_largest_calls(lib):
+    """A launch has less than 2^32 threads; what would need more is refused, not left to the launch."""
+    one = dict(num_heads=1, num_kv_heads=1)
+    for n, rc in (((1 << 26) - 4, SMOE_OK), ((1 << 26) - 3, SMOE_ERR_SHAPE)):
+        assert lib.call("qk_norm_rope", qk(n_rows=n, **one)) == rc
+        for name in ("kv4_append", "kv4_read"):
+            assert lib.call(name, cache(num_kv_heads=1, head_dim=64), rows(n_rows=n)) == rc
+    for more, rc in ((dict(q_rows=(1 << 24) - 1), SMOE_OK), (dict(q_rows=1 << 24), SMOE_ERR_SHAPE),
+                     (dict(n_seqs=(1 << 19) - 9), SMOE_OK), (dict(n_seqs=(1 << 19) - 8), SMOE_ERR_SHAPE),
+                     (dict(k_rows=1 << 28), SMOE_OK), (dict(k_rows=1 << 28, type=smoe_amd.TYPE_F32), SMOE_ERR_SHAPE)):
+        assert lib.call("attention_prompt", prompt(**more)) == rc
+    for n, rc in (((1 << 19) - 1, SMOE_OK), (1 << 19, SMOE_ERR_SHAPE)):
+        assert lib.call("attention_kv4", cache(), attn(n_seqs=n)) == rc
+
+
 def test_lengths_of_an_append(lib):
     assert lib.call("kv4_append", cache(), rows(lens_out=DEV + 8)) == SMOE_OK
     for at in (DEV, DEV + 4, DEV - 4):
