@@ -101,8 +101,7 @@ __device__ __forceinline__ float add2(uint32_t w, float c)
     }
 }
 
-// The sequence of row tile `tile` (ROWS rows each), by the whole wave; false past the last one.
-// Sequences whose offsets point outside their rows have no tiles.
+// a tile's sequence
 struct PromptSeq {
     int32_t q0, nq, k0, nk;
     uint32_t local;                             // tile of the sequence
@@ -128,30 +127,47 @@ __device__ __forceinline__ uint32_t plane_tiles(const PromptLane& s)
 {
     return s.ok && s.z > s.a ? (static_cast<uint32_t>(s.kz - s.ka) + PLANE_KEYS - 1) / PLANE_KEYS : 0;
 }
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, PromptSeq& s)
+// The sequence of tile `tile`, of ROWS (query, head) rows each or (KEYS) of PLANE_KEYS keys, by the whole wave; false past
+// the last one.  Sequences whose offsets point outside their rows have no tiles.  U passes of 64 sequences have their
+// loads in flight at once (4000 sequences of 5 tokens: 558 us against 678 with one).
+template <int ROWS, bool KEYS, bool PLANES, int U>
+__device__ __forceinline__ bool find_tile_by(const PromptAttn& p, uint32_t tile, int lane, bool flag, PromptSeq& s)
 {
     uint32_t base = 0, kbase = 0;
-    for (uint32_t i = 0; i < p.n_seqs; i += WAVE) {
-        const PromptLane l = load_seq(p, i, lane);
-        if (tile == 0 && i + lane < p.n_seqs && !l.ok) flag_range(p.err);
-        const uint32_t n = l.ok ? (static_cast<uint32_t>(l.z - l.a) * p.group + ROWS - 1) / ROWS : 0, kn = plane_tiles(l);
-        const uint32_t upto = base + wave_scan(n), kupto = kbase + wave_scan(kn);
-        const uint64_t past = __ballot(upto > tile);
-        if (past) {
-            const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            s.q0 = __builtin_amdgcn_readlane(l.a, f);
-            s.nq = __builtin_amdgcn_readlane(l.z, f) - s.q0;
-            s.k0 = __builtin_amdgcn_readlane(l.ka, f);
-            s.nk = __builtin_amdgcn_readlane(l.kz, f) - s.k0;
-            s.local = tile - (readlane_u32(upto, f) - readlane_u32(n, f));
-            s.ktile = readlane_u32(kupto, f) - readlane_u32(kn, f);
-            return true;
+    for (uint32_t i = 0; i < p.n_seqs; i += U * WAVE) {
+        PromptLane ls[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) ls[u] = load_seq(p, i + u * WAVE, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const PromptLane& l = ls[u];
+            if (flag && i + u * WAVE + lane < p.n_seqs && !l.ok) flag_range(p.err);
+            const uint32_t n = l.ok ? (static_cast<uint32_t>(l.z - l.a) * p.group + ROWS - 1) / ROWS : 0;
+            const uint32_t kn = PLANES ? plane_tiles(l) : 0, upto = KEYS ? 0 : base + wave_scan(n),
+                           kupto = PLANES ? kbase + wave_scan(kn) : 0;
+            const uint64_t past = __ballot((KEYS ? kupto : upto) > tile);
+            if (past) {
+                const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                s.q0 = __builtin_amdgcn_readlane(l.a, f);
+                s.nq = __builtin_amdgcn_readlane(l.z, f) - s.q0;
+                s.k0 = __builtin_amdgcn_readlane(l.ka, f);
+                s.nk = __builtin_amdgcn_readlane(l.kz, f) - s.k0;
+                s.ktile = readlane_u32(kupto, f) - readlane_u32(kn, f);
+                s.local = tile - (KEYS ? s.ktile : readlane_u32(upto, f) - readlane_u32(n, f));
+                return true;
+            }
+            base = readlane_u32(upto, WAVE - 1);
+            kbase = readlane_u32(kupto, WAVE - 1);
         }
-        base = readlane_u32(upto, WAVE - 1);
-        kbase = readlane_u32(kupto, WAVE - 1);
     }
     return false;
+}
+template <int ROWS, bool KEYS, bool PLANES>
+__device__ __forceinline__ bool find_tile(const PromptAttn& p, uint32_t tile, int lane, PromptSeq& s)
+{
+    const bool flag = !KEYS && blockIdx.x == 0;
+    return p.n_seqs <= WAVE ? find_tile_by<ROWS, KEYS, PLANES, 1>(p, tile, lane, flag, s)
+                            : find_tile_by<ROWS, KEYS, PLANES, 4>(p, tile, lane, flag, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -169,24 +185,10 @@ void k_prompt_planes(PromptAttn p)
     __shared__ uint32_t tops[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t tile = blockIdx.x, kvh = blockIdx.y;
-    // the tile's sequence
-    int32_t k0 = -1, nk = 0;
-    uint32_t local = 0, base = 0;
-    for (uint32_t i = 0; i < p.n_seqs && k0 < 0; i += WAVE) {
-        const PromptLane l = load_seq(p, i, lane);
-        const uint32_t n = plane_tiles(l), upto = base + wave_scan(n);
-        const uint64_t past = __ballot(upto > tile);
-        if (past) {
-            const int f = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            k0 = __builtin_amdgcn_readlane(l.ka, f);
-            nk = __builtin_amdgcn_readlane(l.kz, f) - k0;
-            local = tile - (readlane_u32(upto, f) - readlane_u32(n, f));
-        }
-        base = readlane_u32(upto, WAVE - 1);
-    }
-    if (k0 < 0) return;
-    const uint32_t keys = min(static_cast<uint32_t>(PLANE_KEYS), nk - local * PLANE_KEYS);
-    const uint64_t row0 = static_cast<uint64_t>(k0) + local * PLANE_KEYS;
+    PromptSeq seq;
+    if (!find_tile<1, true, true>(p, tile, lane, seq)) return;
+    const uint32_t keys = min(static_cast<uint32_t>(PLANE_KEYS), seq.nk - seq.local * PLANE_KEYS);
+    const uint64_t row0 = static_cast<uint64_t>(seq.k0) + seq.local * PLANE_KEYS;
     float x[2][PT][8];
     uint32_t top[2] = {0, 0};
 #pragma unroll
@@ -267,7 +269,7 @@ void k_attn_prompt(PromptAttn p)
         tile = blockIdx.x / nkv;
     }
     PromptSeq seq;
-    if (!find_tile<ROWS>(p, tile, lane, seq)) return;
+    if (!find_tile<ROWS, false, S::F32>(p, tile, lane, seq)) return;
     const int32_t q0 = seq.q0, nq = seq.nq, k0 = seq.k0, nk = seq.nk;
     // (sequences that share keys, around one whose offsets are wrong: more key tiles than the scratch holds)
     if (S::F32 && static_cast<uint64_t>(seq.ktile) + static_cast<uint32_t>(nk + PLANE_KEYS - 1) / PLANE_KEYS > p.plane_tiles)

@@ -148,38 +148,51 @@ struct CachePlace {
     bool in_seq, ok;       // the row is of a sequence; its place is in the cache
     bool later;            // a later sequence of the call names the same place
 };
-// Sequence, slot and position of a row, by the whole wave; `near` holds the 64 sequences from i0 on.
-__device__ __forceinline__ CachePlace place_of_row(const Kv4Rows& p, uint32_t row, int lane)
+// Sequence, slot and position of a row, by the whole wave; U passes of 64 sequences have their loads in flight at once
+// (4000 appended rows of 4000 sequences: 24 us against 26 with one)
+template <int U>
+__device__ __forceinline__ CachePlace place_by(const Kv4Rows& p, uint32_t row, int lane)
 {
     CachePlace c{};
     uint32_t seq = 0;
     // (without offsets row r is sequence r's)
-    for (uint32_t i = p.offsets ? 0u : row / WAVE * WAVE; i < p.n_seqs; i += WAVE) {
-        const CallSeqs s = load_seqs(p, i, lane);
-        if (!c.in_seq) {
-            // the first sequence that ends behind the row
-            const uint64_t after = __ballot(s.end > static_cast<int32_t>(row) && i + lane < p.n_seqs);
-            if (!after) continue;
-            const int f = __ffsll(static_cast<unsigned long long>(after)) - 1;
-            seq = i + f;
-            const int32_t at = static_cast<int32_t>(row) - __builtin_amdgcn_readlane(s.first, f);
-            if (at < 0) return c;
-            c.in_seq = true;
-            c.slot = __builtin_amdgcn_readlane(s.slot, f);
-            c.pos = static_cast<uint32_t>(__builtin_amdgcn_readlane(s.start, f)) + static_cast<uint32_t>(at);
-            c.ok = c.slot < p.c.n_slots && c.pos < p.c.capacity;
-            if (!c.ok) {
-                if (lane == 0) flag_range(p.err);
-                return c;
+    for (uint32_t i0 = p.offsets ? 0u : row / WAVE * WAVE; i0 < p.n_seqs; i0 += U * WAVE) {
+        CallSeqs ss[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) ss[u] = load_seqs(p, i0 + u * WAVE, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const CallSeqs& s = ss[u];
+            const uint32_t i = i0 + u * WAVE;
+            if (!c.in_seq) {
+                // the first sequence that ends behind the row
+                const uint64_t after = __ballot(s.end > static_cast<int32_t>(row) && i + lane < p.n_seqs);
+                if (!after) continue;
+                const int f = __ffsll(static_cast<unsigned long long>(after)) - 1;
+                seq = i + f;
+                const int32_t at = static_cast<int32_t>(row) - __builtin_amdgcn_readlane(s.first, f);
+                if (at < 0) return c;
+                c.in_seq = true;
+                c.slot = __builtin_amdgcn_readlane(s.slot, f);
+                c.pos = static_cast<uint32_t>(__builtin_amdgcn_readlane(s.start, f)) + static_cast<uint32_t>(at);
+                c.ok = c.slot < p.c.n_slots && c.pos < p.c.capacity;
+                if (!c.ok) {
+                    if (lane == 0) flag_range(p.err);
+                    return c;
+                }
+                if (!p.slots) return c;
             }
-            if (!p.slots) return c;
+            // (a lane without a sequence of its own has first = end)
+            c.later = __ballot(i + lane > seq && static_cast<uint32_t>(s.slot) == c.slot &&
+                               c.pos - static_cast<uint32_t>(s.start) < static_cast<uint32_t>(s.end - s.first)) != 0;
+            if (c.later) return c;
         }
-        // (a lane without a sequence of its own has first = end)
-        c.later = __ballot(i + lane > seq && static_cast<uint32_t>(s.slot) == c.slot &&
-                           c.pos - static_cast<uint32_t>(s.start) < static_cast<uint32_t>(s.end - s.first)) != 0;
-        if (c.later) return c;
     }
     return c;
+}
+__device__ __forceinline__ CachePlace place_of_row(const Kv4Rows& p, uint32_t row, int lane)
+{
+    return p.n_seqs <= WAVE ? place_by<1>(p, row, lane) : place_by<4>(p, row, lane);
 }
 
 // eight lanes' group of 64 values to its place
