@@ -448,7 +448,10 @@ void k_attn_prompt(PromptAttn p)
                 for (int i = 0; i < 16; ++i) acc[d][i] *= f;
             mx = mn;
         }
-        const float mc = mx > -INFINITY ? mx : 0.f;             // (no key yet: every weight 0)
+        // f16: weights 2^15 times as large, sum and acc with them, or those under 2^-14 of the largest would lose
+        // bits (thousands of them may make up the sum)
+        constexpr float LIFT = __is_same(T, _Float16) ? 15.f : 0.f;
+        const float mc = (mx > -INFINITY ? mx : 0.f) - LIFT;    // (no key yet: every weight 0)
         const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, 15 + vpower - pw.y) : 1.f;
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)

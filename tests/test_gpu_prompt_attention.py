@@ -101,6 +101,26 @@ def test_large_scores(ctx, t):
     assert worst(out, ref, tol) <= 1.0
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("n,over", [(8000, 10.4), (8000, 14.0), (300, 12.0)])
+def test_many_small_weights_beside_a_large_one(ctx, t, n, over):
+    """Weights e^-over each beside one of 1: in f16 far below its normal numbers, together a good part of the sum."""
+    g = gen(n)
+    q, k, v = (torch.zeros(m, 128, device="cuda") for m in (40, n, n))
+    q[:, 0], k[5, 0] = 4.0, over / 4.0
+    q[:, 1:], k[:, 1:] = randn(g, 40, 127, std=0.3), randn(g, n, 127, std=0.02)
+    v.copy_(1.0 + randn(g, n, 128, std=0.2))
+    v[5] = -1.0
+    q, k, v = (x.to(DT[t]) for x in (q, k, v))
+    out = torch.empty_like(q)
+    ctx.attention_prompt(prompt_args(q, k, v, out, i32([0, 40]), i32([0, n]), 1, 1, 128, t, 1.0, n))
+    ctx.synchronize()
+    ref, tol = prompt64(q, k, v, [40], [n], 0, 0, 1, 1, 128, 1.0, t)
+    e = worst(out, ref, tol)
+    print(f"prompt {n} keys, one {over} above, {t}: error / bound {e:.3f}")
+    assert e <= 1.0
+
+
 def test_not_a_number_stays_in_its_sequence(ctx):
     nq = [70, 40, 30]
     q, k, v, out, qo, ko = make(nq, nq, 4, 2, 128, "bf16", 2)
