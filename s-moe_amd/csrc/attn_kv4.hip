@@ -158,6 +158,11 @@ __device__ __forceinline__ uint32_t kv4_parts(uint32_t tiles, uint32_t part)
     const uint32_t c = static_cast<uint32_t>(static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(part)));
     return c * part < tiles ? c + 1 : c;
 }
+// a / b, off by less than 2 or 2^-18 of itself (three roundings, each under 2^-22)
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b)
+{
+    return static_cast<uint32_t>(static_cast<float>(a) * __builtin_amdgcn_rcpf(static_cast<float>(b)));
+}
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) { return readlane_u32(wave_scan(v), WAVE - 1); }
 // tiles of a part; s: the lane's sequence of the first 64; flag: says so if one of the others is out of range
 __device__ __forceinline__ uint32_t kv4_part_tiles(const Kv4Attn& p, int lane, const Kv4Seq& s, bool flag)
@@ -168,10 +173,11 @@ __device__ __forceinline__ uint32_t kv4_part_tiles(const Kv4Attn& p, int lane, c
         total += wave_total(t);
         top = max(top, wave_max_u32(t));
     }
-    // (a tile a wave, and no more parts than the join takes)
-    uint32_t lo = max(max(static_cast<uint32_t>(KA_WAVES), (top + JOIN_MAX - 1) / JOIN_MAX), (total + p.units - 1) / p.units);
+    // (a tile a wave, and no more parts than the join takes; lo may be one less than total / units)
+    uint32_t lo = max(max(static_cast<uint32_t>(KA_WAVES), (top + JOIN_MAX - 1) / JOIN_MAX), quotient(total, p.units));
     // enough at any rate: total / part + one a sequence
-    uint32_t hi = max(lo, p.units > p.n_seqs ? (total + p.units - p.n_seqs - 1) / (p.units - p.n_seqs) : top);
+    const uint32_t q = quotient(total, p.units - p.n_seqs);
+    uint32_t hi = max(lo, min(q + (q >> 18) + 2, top));
     if (p.n_seqs > WAVE) return hi;
     while (lo < hi) {
         const uint32_t mid = (lo + hi) / 2;
@@ -179,6 +185,13 @@ __device__ __forceinline__ uint32_t kv4_part_tiles(const Kv4Attn& p, int lane, c
         else lo = mid + 1;
     }
     return lo;
+}
+
+// behind the parts in the scratch: first part and number of parts of every sequence
+template <int HD>
+__device__ __forceinline__ uint2* kv4_info(const Kv4Attn& p)
+{
+    return reinterpret_cast<uint2*>(p.part + part_floats(static_cast<size_t>(p.units) * p.c.num_kv_heads * p.group, 1, HD));
 }
 
 template <int HD, typename T>
@@ -206,6 +219,15 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
     if (p.units) {
         Kv4Seq s = kv4_seq(p, lane, blockIdx.x == 0);
         const uint32_t part = kv4_part_tiles(p, lane, s, blockIdx.x == 0);
+        if (blockIdx.x == 0 && wv == 0) {                       // for the join: each sequence's first part and parts
+            Kv4Seq z = s;
+            for (uint32_t i = 0, base = 0; i < p.n_seqs; i += WAVE) {
+                if (i) z = kv4_seq(p, i + lane, false);
+                const uint32_t c = kv4_parts(z.tiles, part), upto = base + wave_scan(c);
+                if (i + lane < p.n_seqs) kv4_info<HD>(p)[i + lane] = make_uint2(upto - c, c);
+                base = readlane_u32(upto, WAVE - 1);
+            }
+        }
         for (uint32_t i = 0, base = 0;;) {
             const uint32_t c = kv4_parts(s.tiles, part), upto = base + wave_scan(c);
             if (const uint64_t past = __ballot(upto > unit)) {
@@ -526,17 +548,8 @@ void k_kv4_join(Kv4Attn p)
     const uint32_t heads = p.c.num_kv_heads * p.group;
     const uint32_t w = blockIdx.x * KA_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seq = w / heads;
     if (seq >= p.n_seqs) return;
-    // the sequence's parts, as its blocks found them
-    Kv4Seq s = kv4_seq(p, lane, false);
-    const uint32_t part = kv4_part_tiles(p, lane, s, false);
-    uint32_t base = 0, c = kv4_parts(s.tiles, part), i = 0;
-    for (; i + WAVE <= seq; i += WAVE) {
-        base += wave_total(c);
-        s = kv4_seq(p, i + WAVE + lane, false);
-        c = kv4_parts(s.tiles, part);
-    }
-    const uint32_t upto = base + wave_scan(c);
-    const uint32_t parts = readlane_u32(c, seq - i), first = readlane_u32(upto, seq - i) - parts;
+    const uint2 info = kv4_info<HD>(p)[seq];
+    const uint32_t first = info.x, parts = info.y;
     if (parts == 1) return;                                     // (its block wrote the row)
     const size_t at = static_cast<size_t>(first) * heads + w % heads;
     float o[HD / WAVE];
@@ -561,7 +574,8 @@ void kv4_plan(Kv4Attn& a, uint32_t head_dim, uint32_t max_len)
 size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t head_dim)
 {
     if (a.units == 0) return 0;
-    return part_floats(static_cast<size_t>(a.units) * a.c.num_kv_heads * a.group, 1, head_dim) * sizeof(float);
+    return part_floats(static_cast<size_t>(a.units) * a.c.num_kv_heads * a.group, 1, head_dim) * sizeof(float) +
+           a.n_seqs * sizeof(uint2);
 }
 
 hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t head_dim, uint32_t type, hipStream_t s)
