@@ -20,6 +20,9 @@
 //     Tiles.  K and V tiles go to LDS by direct loads, one tile ahead, in 16-byte
 //     pieces whose place in a row is exchanged (kswz, vswz) so that the operand reads
 //     meet no bank twice: K as 16-byte pieces of 32 rows, V by transposing reads of 8 rows.
+//     Order.  LDS operands are requested a few products ahead, and the weights of 16 keys
+//     are formed between the products of the 16 before (sched_group_barrier; left to the
+//     compiler 1 to 5 % slower).
 //     16-bit types: v_mfma_f32_32x32x16 with P rounded to their type (the weights' sum is
 //     of the rounded ones, in fp32).  f32: every operand as two f16 (hi + lo, 22 bits) and
 //     three products for one, 16 / 3 times the rate of the fp32 MFMA.  K and V are split
@@ -389,6 +392,9 @@ void k_attn_prompt(PromptAttn p)
     int vpower = NO_POWER;                                      // f32: acc holds the sum times 2^(15 + vpower)
     const int2* powers = S::F32 ? p.powers + static_cast<size_t>(kvh) * p.plane_tiles + seq.ktile : nullptr;
 
+    // K operands requested ahead, and whether those of V are, as far as registers go
+    constexpr int SA = S::F32 ? 2 : 4;
+    constexpr bool VAHEAD = !S::F32 || HD < 128;
     auto tile_step = [&](int32_t t, int b, int2 pw) {
         const uint8_t* kl = mine + b * S::BUF;
         const uint8_t* vl = kl + S::PLANES * S::TILE;
@@ -398,18 +404,50 @@ void k_attn_prompt(PromptAttn p)
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+        auto kop = [&](int i, int pl) {
+            const int ks = i / NSUB, u = i % NSUB;
+            return *reinterpret_cast<const uint4*>(kl + pl * S::TILE + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col)));
+        };
+        // place c of a 16-lane group of a transposing read names row c / 4 and dims 4 (c % 4) .. of 16;
+        // the lane receives the rows' values of dim c
+        const int c = lane & 15;
+        auto vop = [&](int ks, int d, int pl) {
+            return read_rows8(vl + pl * S::TILE + (16 * ks + 4 * h + (c >> 2)) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
+                              32 * ((lane >> 4) & 1) + 8 * (c & 3), RB);
+        };
+        uint4 va[2][ND][S::PLANES];
+        constexpr int NK = QN * NSUB;
 #pragma unroll
-        for (int ks = 0; ks < QN; ++ks)
-#pragma unroll
-            for (int u = 0; u < NSUB; ++u) {
-                const uint8_t* at = kl + (u * 32 + col) * RB + 16 * ((2 * ks + h) ^ S::kswz(col));
-                const uint4 a = *reinterpret_cast<const uint4*>(at);
-                s[u] = mma16<M>(a, qf[0][ks], s[u]);
-                if constexpr (S::F32) {
-                    s[u] = mma16<M>(a, qf[1][ks], s[u]);
-                    s[u] = mma16<M>(*reinterpret_cast<const uint4*>(at + S::TILE), qf[0][ks], s[u]);
-                }
+        for (int i = 0; i < NK; ++i) {
+            const int ks = i / NSUB, u = i % NSUB;
+            const uint4 a = kop(i, 0);
+            s[u] = mma16<M>(a, qf[0][ks], s[u]);
+            if constexpr (S::F32) {
+                s[u] = mma16<M>(a, qf[1][ks], s[u]);
+                s[u] = mma16<M>(kop(i, 1), qf[0][ks], s[u]);
             }
+        }
+        auto ahead = [&](int ks) {
+            if constexpr (VAHEAD)
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int pl = 0; pl < S::PLANES; ++pl) va[ks & 1][d][pl] = vop(ks, d, pl);
+        };
+        ahead(0);
+        // the order: SA operands, then one for each that the products have taken, then the first of V
+        // (0x100 LDS reads, 0x8 MFMA, 0x402 VALU with the transcendentals)
+        __builtin_amdgcn_sched_group_barrier(0x100, SA * S::PLANES, 0);
+#pragma unroll
+        for (int i = 0; i < NK - SA; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, S::F32 ? 3 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, S::PLANES, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < SA; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, S::F32 ? 3 : 1, 0);
+            if (VAHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 2 * ND * S::PLANES / SA, 0);
+        }
         float sc = c2;
         if constexpr (S::F32) {
             // (never 0: a hidden key's -inf stays one)
@@ -453,45 +491,59 @@ void k_attn_prompt(PromptAttn p)
         constexpr float LIFT = __is_same(T, _Float16) ? 15.f : 0.f;
         const float mc = (mx > -INFINITY ? mx : 0.f) - LIFT;    // (no key yet: every weight 0)
         const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, 15 + vpower - pw.y) : 1.f;
+        // ---- weights of 16 keys, and O^T += V^T P^T of the 16 before ----
+        uint4 pb[2], pl[2];
+        auto weights = [&](int ks) {
+            f32x16_t& sv = s[ks / 2];
+            const int o = (ks % 2) * 8;
 #pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], sc, -mc));
+            for (int i = o; i < o + 8; ++i) {
+                sv[i] = __builtin_amdgcn_exp2f(fmaf(sv[i], sc, -mc));
                 if constexpr (S::F32) {
-                    sum += s[u][i];
-                    s[u][i] *= pf;
+                    sum += sv[i];
+                    sv[i] *= pf;
                 }
             }
-        // ---- O^T += V^T P^T ----
-        // place c of a 16-lane group of a transposing read names row c / 4 and dims 4 (c % 4) .. of 16;
-        // the lane receives the rows' values of dim c
-        const int c = lane & 15, vrow = 4 * h + (c >> 2);
+            uint4& w = pb[ks & 1];
+            if constexpr (S::F32) {
+                uint4& l = pl[ks & 1];
+                split2(sv[o + 0], sv[o + 1], w.x, l.x);
+                split2(sv[o + 2], sv[o + 3], w.y, l.y);
+                split2(sv[o + 4], sv[o + 5], w.z, l.z);
+                split2(sv[o + 6], sv[o + 7], w.w, l.w);
+            } else {
+                w = make_uint4(pack2<T>(sv[o + 0], sv[o + 1]), pack2<T>(sv[o + 2], sv[o + 3]),
+                               pack2<T>(sv[o + 4], sv[o + 5]), pack2<T>(sv[o + 6], sv[o + 7]));
+                sum = add2<T>(w.x, add2<T>(w.y, add2<T>(w.z, add2<T>(w.w, sum))));
+            }
+        };
+        weights(0);
+        if constexpr (VAHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KT / 16; ++ks) {
-            uint4 pb, pl;
-            const f32x16_t& sv = s[ks / 2];
-            const int o = (ks % 2) * 8;
-            if constexpr (S::F32) {
-                split2(sv[o + 0], sv[o + 1], pb.x, pl.x);
-                split2(sv[o + 2], sv[o + 3], pb.y, pl.y);
-                split2(sv[o + 4], sv[o + 5], pb.z, pl.z);
-                split2(sv[o + 6], sv[o + 7], pb.w, pl.w);
-            } else {
-                pb = make_uint4(pack2<T>(sv[o + 0], sv[o + 1]), pack2<T>(sv[o + 2], sv[o + 3]),
-                                pack2<T>(sv[o + 4], sv[o + 5]), pack2<T>(sv[o + 6], sv[o + 7]));
-                sum = add2<T>(pb.x, add2<T>(pb.y, add2<T>(pb.z, add2<T>(pb.w, sum))));
+            if (ks + 1 < KT / 16) {
+                ahead(ks + 1);
+                weights(ks + 1);
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const uint8_t* at = vl + (16 * ks + vrow) * RB + 16 * ((4 * d) ^ S::vswz(c >> 2)) +
-                                    32 * ((lane >> 4) & 1) + 8 * (c & 3);
-                const uint4 a = read_rows8(at, RB);
+                const uint4 a = VAHEAD ? va[ks & 1][d][0] : vop(ks, d, 0);
                 if constexpr (S::F32) {
-                    acc[d] = mma16<M>(a, pl, acc[d]);
-                    acc[d] = mma16<M>(read_rows8(at + S::TILE, RB), pb, acc[d]);
+                    acc[d] = mma16<M>(a, pl[ks & 1], acc[d]);
+                    acc[d] = mma16<M>(VAHEAD ? va[ks & 1][d][S::PLANES - 1] : vop(ks, d, 1), pb[ks & 1], acc[d]);
                 }
-                acc[d] = mma16<M>(a, pb, acc[d]);
+                acc[d] = mma16<M>(a, pb[ks & 1], acc[d]);
+            }
+            if constexpr (VAHEAD) {
+                if (ks + 1 < KT / 16) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * ND * S::PLANES, 0);
+#pragma unroll
+                    for (int d = 0; d < ND * (S::F32 ? 3 : 1); ++d) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
