@@ -395,6 +395,11 @@ void k_attn_prompt(PromptAttn p)
     // K operands requested ahead, and whether those of V are, as far as registers go
     constexpr int SA = S::F32 ? 2 : 4;
     constexpr bool VAHEAD = !S::F32 || HD < 128;
+    // The sums are rescaled when a row's maximum has grown by more than 2^SLACK, not whenever it has: with 32 rows a
+    // wave one of them has a new maximum in every other tile.  Weights may then be up to 2^SLACK, which 16-bit types
+    // hold as well as 1 (f32: no slack, its f16 halves have no room).  f16: weights 2^LIFT times as large, sum and acc
+    // with them, or those under 2^-14 would be subnormal and lose bits (thousands of them may make up the sum).
+    constexpr float SLACK = S::F32 ? 0.f : 8.f, LIFT = __is_same(T, _Float16) ? 7.f : 0.f;
     auto tile_step = [&](int32_t t, int b, int2 pw) {
         const uint8_t* kl = mine + b * S::BUF;
         const uint8_t* vl = kl + S::PLANES * S::TILE;
@@ -471,7 +476,7 @@ void k_attn_prompt(PromptAttn p)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[u][i]);
         mt = half_max(mt) * sc;
-        if (__ballot(mt > mx) || (S::F32 && pw.y < vpower)) {
+        if (__ballot(mt > mx + SLACK) || (S::F32 && pw.y < vpower)) {
             const float mn = fmaxf(mx, mt);
             float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 0.f;
             sum *= f;
@@ -486,9 +491,6 @@ void k_attn_prompt(PromptAttn p)
                 for (int i = 0; i < 16; ++i) acc[d][i] *= f;
             mx = mn;
         }
-        // f16: weights 2^15 times as large, sum and acc with them, or those under 2^-14 of the largest would lose
-        // bits (thousands of them may make up the sum)
-        constexpr float LIFT = __is_same(T, _Float16) ? 15.f : 0.f;
         const float mc = (mx > -INFINITY ? mx : 0.f) - LIFT;    // (no key yet: every weight 0)
         const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, 15 + vpower - pw.y) : 1.f;
         // ---- weights of 16 keys, and O^T += V^T P^T of the 16 before ----
