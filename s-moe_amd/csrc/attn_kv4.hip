@@ -357,6 +357,9 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
     const uint32_t kat = m16 * RB + (((q >> 1) ^ S::swz(m16)) * 16) + (q & 1) * 8;
     const uint32_t vrow = 16 * ((m16 >> 2) & 1) + 4 * q + (m16 & 3);
     const uint32_t vat = vrow * RB + (S::swz(vrow) * 16) + (m16 >> 3) * 8;
+    // the sums are rescaled when a head's maximum has grown by more than 2^SLACK: weights up to that
+    constexpr float SLACK = 4.f;
+    constexpr int VLIFT = 10;
     auto step = [&](uint32_t t, int b0) {
         const uint8_t* kl = mine + b0 * S::BUF;
         const uint8_t* vl = kl + S::CODES;
@@ -431,7 +434,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
             grown |= eb[g] != ebits[g];
             e = lane % NG == g ? eb[g] : e;
         }
-        if (__ballot(mt > mx) || grown) {
+        if (__ballot(mt > mx + SLACK) || grown) {
             const float mn = fmaxf(mx, mt);
             const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 0.f;
             sum *= f;
@@ -445,7 +448,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
             }
             mx = mn;
         }
-        put_pairs(vp, __builtin_amdgcn_ldexpf(1.f, 127 + 14 - e));     // P times a scale stays under 2^15
+        put_pairs(vp, __builtin_amdgcn_ldexpf(1.f, 127 + VLIFT - e));  // P times a scale stays under 2^15
         const float m0 = mx > -INFINITY ? mx : 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -501,7 +504,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         vmin[g] = quads_sum(vmin[g]);
-        const float down = __builtin_amdgcn_ldexpf(1.f, ebits[g] - 127 - 14);
+        const float down = __builtin_amdgcn_ldexpf(1.f, ebits[g] - 127 - VLIFT);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
             *reinterpret_cast<float4*>(buf + (wv * KA_HEADS + m16) * RS + 64 * g + 16 * d + 4 * q) =
