@@ -529,7 +529,7 @@ typedef struct {
     const int32_t* offsets;         /* [n_seqs + 1] or NULL */
     const int32_t* slots;           /* [n_seqs] or NULL */
     const int32_t* start;           /* [n_seqs] */
-    int32_t*       lens_out;        /* append: [n_seqs] start + rows, or NULL; not start itself */
+    int32_t*       lens_out;        /* append: [n_seqs] start + rows, or NULL; a buffer of its own */
     uint64_t k_stride, v_stride;
     uint32_t n_seqs, n_rows, type;
 } SmoeKv4RowsArgs;
@@ -541,7 +541,7 @@ int smoe_hip_kv4_read(SmoeMetalCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv
 
 /* Attention of one token a sequence (GQA, decode.cpp:190-227) over the first
  * lens[b] positions of slot slots[b]: out [n_seqs x num_heads x head_dim] from q
- * of the same shape; lens[b] = 0 gives zeros.  max_len: the longest length as far
+ * of the same shape (out may be q, with its stride); lens[b] = 0 gives zeros.  max_len: the longest length as far
  * as known, 0: capacity; it only decides how the work is split (a captured graph
  * follows lens). */
 typedef struct {

@@ -245,9 +245,12 @@ extern "C" int smoe_hip_kv4_append(SmoeMetalCtx* ctx, const SmoeKv4Cache* c, con
 {
     if (!ctx) return SMOE_ERR_ARG;
     if (const int rc = check_kv4_rows(ctx, c, a)) return rc;
-    // other blocks still read start when the first one writes the lengths
-    if (a->lens_out && a->lens_out < a->start + a->n_seqs && a->start < a->lens_out + a->n_seqs)
-        return refuse(ctx, SMOE_ERR_ARG, "lens_out overlaps start");
+    // other blocks still read these when the first one writes the lengths
+    auto overlaps = [&](const int32_t* p, uint64_t n) {
+        return a->lens_out && p && a->lens_out < p + n && p < a->lens_out + a->n_seqs;
+    };
+    if (overlaps(a->start, a->n_seqs) || overlaps(a->slots, a->n_seqs) || overlaps(a->offsets, uint64_t(a->n_seqs) + 1))
+        return refuse(ctx, SMOE_ERR_ARG, "lens_out overlaps start, slots or offsets");
     const smoe::ContextView v = smoe::context_view(ctx);
     const OnDevice on(v.device);
     if (!on.ok()) return refuse(ctx, SMOE_ERR_HIP, "hipSetDevice failed");

@@ -174,10 +174,14 @@ def test_the_largest_calls(lib):
 
 
 def test_lengths_of_an_append(lib):
-    assert lib.call("kv4_append", cache(), rows(lens_out=DEV + 8)) == SMOE_OK
+    assert lib.call("kv4_append", cache(), rows(lens_out=DEV + 64)) == SMOE_OK
     for at in (DEV, DEV + 4, DEV - 4):
         assert lib.call("kv4_append", cache(), rows(lens_out=at)) == SMOE_ERR_ARG
-    assert lib.call("kv4_read", cache(), rows(lens_out=DEV + 8)) == SMOE_ERR_ARG
+    apart = dict(start=DEV, slots=DEV + 64, offsets=DEV + 128)         # 2, 2 and 3 words
+    for at, rc in ((4, SMOE_ERR_ARG), (8, SMOE_OK), (60, SMOE_ERR_ARG), (68, SMOE_ERR_ARG), (72, SMOE_OK), (120, SMOE_OK),
+                   (124, SMOE_ERR_ARG), (136, SMOE_ERR_ARG), (140, SMOE_OK)):
+        assert lib.call("kv4_append", cache(), rows(lens_out=DEV + at, **apart)) == rc
+    assert lib.call("kv4_read", cache(), rows(lens_out=DEV + 64)) == SMOE_ERR_ARG
 
 
 @pytest.mark.parametrize("more,rc", [
@@ -215,7 +219,7 @@ def test_calls_without_rows_do_nothing(lib):
     assert L.smoe_hip_kv4_read(lib.ctx, C.byref(cache()), C.byref(rows(n_rows=0))) == SMOE_OK
     assert lib.booked() == n
     # (the lengths are still wanted)
-    assert lib.call("kv4_append", cache(), rows(n_rows=0, lens_out=DEV + 8)) == SMOE_OK
+    assert lib.call("kv4_append", cache(), rows(n_rows=0, lens_out=DEV + 64)) == SMOE_OK
 
 
 def test_scratch_grows_outside_capture_only(lib):

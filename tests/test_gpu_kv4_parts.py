@@ -96,6 +96,24 @@ def test_the_hint_may_be_wrong(ctx, max_len):
     assert worst(out, ref, tol) <= 1.0
 
 
+def test_in_place(ctx):
+    """out may be q: a row's blocks have read it before anyone writes it."""
+    g = gen(10)
+    lens = [2500, 1, 40, 0, 900]
+    cache = Cache(g, 5, 2, 2500, 128)
+    q = randn(g, 5, 40 * 128)
+    want = run(ctx, cache, q, lens, range(5), 40, "f32", 2500)
+    for max_len in (2500, 100):                  # in parts, and each sequence whole
+        x = q.clone()
+        ctx.attention_kv4(cache.struct(), kv4_args(x, x, i32(lens), 40, "f32", 0.09, None, max_len))
+        ctx.synchronize()
+        if max_len == 2500:
+            assert torch.equal(x, want)
+        else:
+            ref, tol = kv4_64(cache, q, lens, range(5), 40, 0.09, "f32")
+            assert worst(x, ref, tol) <= 1.0
+
+
 def test_all_empty(ctx):
     g = gen(8)
     cache = Cache(g, 4, 2, 3000, 128)
