@@ -99,6 +99,7 @@ struct Kv4Attn {
     float scale_log2;
     uint32_t units;             // parts of all sequences' positions for a KV head, joined by a second launch;
                                 // 0: each sequence whole
+    uint32_t waves;             // of a block: 4 or 8
     float* part;                // rows = units times heads (part_floats, one part a row)
     uint32_t* err;
 };

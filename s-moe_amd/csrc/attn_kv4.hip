@@ -4,7 +4,7 @@
 //   k_j = c s_g + m_g in groups of 64 dims, codes c of 0 .. 15
 //
 //   k_attn_kv4   one block per (sequence, KV head, up to 16 of its query heads, part of
-//                the positions), four waves that take tiles of 32 positions in turn and
+//                the positions), four or eight waves that take tiles of 32 positions in turn and
 //                are merged in LDS.
 //     Codes go through v_mfma_f32_16x16x32_f16 as they are: 0 .. 15 are exact in f16
 //     (two codes a word by one and-or with the bits of 1024 or 64 and one packed
@@ -28,9 +28,9 @@
 //     twice.  The 16 lanes that share a position would unpack the same scales and mins, so
 //     each pair is put into floats by one lane and passed on through LDS.
 //     Bound: the cache's bytes where there are many (head_dim 128, 4 KV heads: 48 sequences of
-//     8192, bf16, 226 MB in 53 us, 4.3 TB/s; 16 of 32768, 64 query heads, f32, 302 MB in
-//     70 us, 4.3 TB/s, of which the loads alone take 58; a large copy reaches 5.1 TB/s), else
-//     the launch and one chain of length, tile and query loads: one sequence of 777, 7 us.
+//     8192, bf16, 226 MB in 51 us, 4.4 TB/s; 16 of 32768, 64 query heads, f32, 302 MB in
+//     66 us, 4.6 TB/s, of which the loads alone take 58; a large copy reaches 5.1 TB/s), else
+//     the launch and one chain of length, tile and query loads: one sequence of 777, 7.5 us.
 //   k_kv4_join   the parts of each (sequence, head) joined (4 us, 5 with 64 parts a row).
 #include <algorithm>
 
@@ -39,8 +39,7 @@
 
 namespace smoe {
 
-constexpr int KA_WAVES = 4;
-constexpr int KA_THREADS = KA_WAVES * WAVE;
+constexpr int KA_JOIN_WAVES = 4;
 constexpr int KA_TILE = 32;             // positions of a wave step
 constexpr int KA_HEADS = 16;            // query heads of a block (MFMA columns)
 
@@ -109,7 +108,7 @@ __device__ __forceinline__ void lds_load4(const void* base, uint32_t off, uint32
 
 // a wave's buffer of one tile: K codes, V codes (rows of RB bytes), then the scale and min
 // words of K and of V as they are, later the floats of one of them
-template <int HD>
+template <int HD, int KW>
 struct Kv4Shape {
     static constexpr int NG = HD / 64;
     static constexpr int RB = HD / 2, PIECES = RB / 16;
@@ -119,7 +118,7 @@ struct Kv4Shape {
     static constexpr int NP = (PAIRS + 63) / 64;               // direct loads of a tile's pairs
     static constexpr int BUF = 2 * CODES + 2 * NP * 256;
     static constexpr int RS = HD + 4;                          // padded row of a head in the merge
-    static constexpr int LDS = KA_WAVES * (2 * BUF > KA_HEADS * RS * 4 ? 2 * BUF : KA_HEADS * RS * 4);
+    static constexpr int LDS = KW * (2 * BUF > KA_HEADS * RS * 4 ? 2 * BUF : KA_HEADS * RS * 4);
     static constexpr int WAVES_PER_SIMD = HD == 256 ? 2 : 4;
     static_assert(2 * PAIRS * 4 <= 2 * NP * 256, "the floats of K or V fit the words' place");
     // piece c of row r stands at piece c ^ swz(r)
@@ -129,7 +128,7 @@ struct Kv4Shape {
 // ---------------------------------------------------------------------------
 // Which positions a block takes.  The sequences' tiles are cut into p.units parts or fewer
 // of the same length, as near as may be, so that sequences of different lengths give every
-// block the same work (32 sequences of up to 8192: 24 us against 26 with the longest one's
+// block the same work (32 sequences of up to 8192, as it was then: 24 us against 26 with the longest one's
 // parts for all): the shortest length at which the parts of all sequences are few enough.
 // Every wave works it out from the lengths, 64 sequences a pass; for more than 64 it takes
 // the length that is enough at any rate.
@@ -174,7 +173,7 @@ __device__ __forceinline__ uint32_t kv4_part_tiles(const Kv4Attn& p, int lane, c
         top = max(top, wave_max_u32(t));
     }
     // (a tile a wave, and no more parts than the join takes; lo may be one less than total / units)
-    uint32_t lo = max(max(static_cast<uint32_t>(KA_WAVES), (top + JOIN_MAX - 1) / JOIN_MAX), quotient(total, p.units));
+    uint32_t lo = max(max(p.waves, (top + JOIN_MAX - 1) / JOIN_MAX), quotient(total, p.units));
     // enough at any rate: total / part + one a sequence
     const uint32_t q = quotient(total, p.units - p.n_seqs);
     uint32_t hi = max(lo, min(q + (q >> 18) + 2, top));
@@ -194,15 +193,15 @@ __device__ __forceinline__ uint2* kv4_info(const Kv4Attn& p)
     return reinterpret_cast<uint2*>(p.part + part_floats(static_cast<size_t>(p.units) * p.c.num_kv_heads * p.group, 1, HD));
 }
 
-template <int HD, typename T>
-__global__ __launch_bounds__(KA_THREADS, (Kv4Shape<HD>::WAVES_PER_SIMD))
+template <int HD, typename T, int KW>
+__global__ __launch_bounds__(KW * WAVE, (Kv4Shape<HD, KW>::WAVES_PER_SIMD))
 void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 {
-    using S = Kv4Shape<HD>;
+    using S = Kv4Shape<HD, KW>;
     constexpr int NG = S::NG, RB = S::RB, RS = S::RS;
     constexpr bool Q2 = sizeof(T) == 4;         // q as two f16
     extern __shared__ __align__(16) float buf[];    // the waves' tiles; before and after, rows of heads
-    __shared__ float qsum[KA_HEADS * NG], mw[KA_WAVES * KA_HEADS], lw[KA_WAVES * KA_HEADS];
+    __shared__ float qsum[KA_HEADS * NG], mw[KW * KA_HEADS], lw[KW * KA_HEADS];
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m16 = lane & 15, q = lane >> 4;
@@ -286,7 +285,7 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 
     // ---- the query heads: a power of two each, then f16 --------------------------
     // (through the waves' second buffers, which the first tile leaves alone)
-    constexpr int HPW = KA_HEADS / KA_WAVES;
+    constexpr int HPW = KA_HEADS / KW;
     static_assert(HPW * RS * 4 <= S::BUF, "a wave's heads fit its second buffer");
     auto head_row = [&](uint32_t g) {
         return reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(buf) + g / HPW * (2 * S::BUF) + S::BUF) + g % HPW * RS;
@@ -491,10 +490,10 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
         }
     };
     int b = 0;
-    for (uint32_t t = t0 + wv; t < t1; t += KA_WAVES, b ^= 1) {
+    for (uint32_t t = t0 + wv; t < t1; t += KW, b ^= 1) {
         // tile t has arrived, and nothing of the other buffer is still being read
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (t + KA_WAVES < t1) issue(t + KA_WAVES, b ^ 1);
+        if (t + KW < t1) issue(t + KW, b ^ 1);
         step(t, b);
     }
 
@@ -516,15 +515,15 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
         lw[wv * KA_HEADS + m16] = sum;
     }
     __syncthreads();
-    for (uint32_t o = threadIdx.x; o < ng * HD; o += KA_THREADS) {
+    for (uint32_t o = threadIdx.x; o < ng * HD; o += KW * WAVE) {
         const uint32_t g = o / HD, d = o % HD, head = hbase + g;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KA_WAVES; ++w) M = fmaxf(M, mw[w * KA_HEADS + g]);
+        for (int w = 0; w < KW; ++w) M = fmaxf(M, mw[w * KA_HEADS + g]);
         const float m0 = M > -INFINITY ? M : 0.f;
         float L = 0.f, A = 0.f;
 #pragma unroll
-        for (int w = 0; w < KA_WAVES; ++w) {
+        for (int w = 0; w < KW; ++w) {
             const float f = __builtin_amdgcn_exp2f(mw[w * KA_HEADS + g] - m0);
             L = fmaf(f, lw[w * KA_HEADS + g], L);
             A = fmaf(f, buf[(w * KA_HEADS + g) * RS + d], A);
@@ -544,12 +543,12 @@ void k_attn_kv4(Kv4Attn p, uint32_t n_sub)
 
 // one wave per (sequence, head)
 template <int HD, typename T>
-__global__ __launch_bounds__(KA_THREADS)
+__global__ __launch_bounds__(KA_JOIN_WAVES * WAVE)
 void k_kv4_join(Kv4Attn p)
 {
     const int lane = threadIdx.x & 63;
     const uint32_t heads = p.c.num_kv_heads * p.group;
-    const uint32_t w = blockIdx.x * KA_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seq = w / heads;
+    const uint32_t w = blockIdx.x * KA_JOIN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seq = w / heads;
     if (seq >= p.n_seqs) return;
     const uint2 info = kv4_info<HD>(p)[seq];
     const uint32_t first = info.x, parts = info.y;
@@ -564,13 +563,23 @@ void k_kv4_join(Kv4Attn p)
 void kv4_plan(Kv4Attn& a, uint32_t head_dim, uint32_t max_len)
 {
     const uint32_t n_sub = (a.group + KA_HEADS - 1) / KA_HEADS;
-    const uint32_t quads = max_len / (KA_WAVES * KA_TILE) + (max_len % (KA_WAVES * KA_TILE) != 0);
-    // As many parts as blocks are resident at once (256 CUs of four, or two at head_dim 256), each with a tile a
-    // wave or more: 16 sequences of 32768 over 4 KV heads 72.8 us in 16 parts (1024 blocks), 78.0 in 8, 74.8
-    // in 12, 76.2 in 24; one of 777 over 4 KV heads 6.9 us in 7 parts, 8.5 in 6, 15.5 in one.  Sequences whole
-    // where they fill half of that, or no sequence has a second part.
-    const uint32_t most = (head_dim == 256 ? 512 : 1024) / (a.c.num_kv_heads * n_sub);
-    a.units = static_cast<uint32_t>(std::min<uint64_t>(most, static_cast<uint64_t>(a.n_seqs) * quads));
+    const uint32_t tiles = max_len / KA_TILE + (max_len % KA_TILE != 0);
+    // As many parts as blocks are resident at once (1024 of four waves, 512 of eight; half at head_dim 256), each with
+    // a tile a wave or more: 16 sequences of 32768 over 4 KV heads 72.8 us in 16 parts (1024 blocks of four waves),
+    // 78.0 in 8, 74.8 in 12, 76.2 in 24; one of 777 over 4 KV heads 6.9 us in 7 parts, 8.5 in 6, 15.5 in one.
+    // Sequences whole where they fill half of that, or no sequence has a second part.
+    auto most = [&](uint32_t waves) { return (head_dim == 256 ? 2048 : 4096) / waves / (a.c.num_kv_heads * n_sub); };
+    auto units = [&](uint32_t waves) {
+        return static_cast<uint32_t>(std::min<uint64_t>(most(waves), static_cast<uint64_t>(a.n_seqs) * ((tiles + waves - 1) / waves)));
+    };
+    // Eight waves a block (half the query set-ups, merges and parts: 16 of 32768 65.4 us against 68.4, 16 of 3000 14.0
+    // against 17.5) where the sequences fill the resident blocks with them, four parts or more each and no more than a
+    // tenth of the blocks left over (48 of 8192 58.8 against 51.2, 64 ragged ones 27.7 against 26.3, one of 777 7.8
+    // against 7.6 and a longer join).
+    const uint32_t m8 = most(8);
+    const bool eight = units(8) == m8 && m8 >= 4 * static_cast<uint64_t>(a.n_seqs) && m8 % a.n_seqs * 10 <= m8;
+    a.waves = eight ? 8 : 4;
+    a.units = units(a.waves);
     if (a.units < 2 * static_cast<uint64_t>(a.n_seqs)) a.units = 0;
 }
 
@@ -581,22 +590,31 @@ size_t kv4_scratch_bytes(const Kv4Attn& a, uint32_t head_dim)
            a.n_seqs * sizeof(uint2);
 }
 
+template <int HD, typename T, int KW>
+static hipError_t launch_kv4(const Kv4Attn& a, uint32_t n_sub, hipStream_t s)
+{
+    constexpr uint32_t lds = Kv4Shape<HD, KW>::LDS;
+    static_assert(lds <= 155 * 1024, "LDS of a CU, beside the static arrays");
+    if constexpr (lds > 60 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_kv4<HD, T, KW>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    launch_kernel_lds(k_attn_kv4<HD, T, KW>, dim3((a.units ? a.units : a.n_seqs) * a.c.num_kv_heads * n_sub), dim3(KW * WAVE),
+                      lds, s, a, n_sub);
+    return hipGetLastError();
+}
+
 hipError_t launch_attention_kv4(const Kv4Attn& a, uint32_t head_dim, uint32_t type, hipStream_t s)
 {
     return with_type_and_head(type, head_dim, [&](auto t, auto hd) {
         constexpr int HD = decltype(hd)::value;
         using T = decltype(t);
         const uint32_t n_sub = (a.group + KA_HEADS - 1) / KA_HEADS, heads = a.c.num_kv_heads * a.group;
-        constexpr uint32_t lds = Kv4Shape<HD>::LDS;
-        if constexpr (lds > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_attn_kv4<HD, T>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e != hipSuccess) return e;
-        }
-        launch_kernel_lds(k_attn_kv4<HD, T>, dim3((a.units ? a.units : a.n_seqs) * a.c.num_kv_heads * n_sub),
-                          dim3(KA_THREADS), lds, s, a, n_sub);
-        if (a.units)
-            launch_kernel(k_kv4_join<HD, T>, dim3((a.n_seqs * heads + KA_WAVES - 1) / KA_WAVES), dim3(KA_THREADS), s, a);
+        const hipError_t e = a.waves == 8 ? launch_kv4<HD, T, 8>(a, n_sub, s) : launch_kv4<HD, T, 4>(a, n_sub, s);
+        if (e != hipSuccess || a.units == 0) return e;
+        launch_kernel(k_kv4_join<HD, T>, dim3((a.n_seqs * heads + KA_JOIN_WAVES - 1) / KA_JOIN_WAVES),
+                      dim3(KA_JOIN_WAVES * WAVE), s, a);
         return hipGetLastError();
     });
 }

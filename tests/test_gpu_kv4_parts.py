@@ -45,6 +45,24 @@ def test_ragged(ctx, n, most, heads, kv, hd, t, hint):
     assert all((out[i] == 0).all() for i in range(n) if lens[i] == 0)
 
 
+@pytest.mark.parametrize("n,most,heads,kv,hd,t", [
+    (8, 4200, 8, 4, 128, "bf16"), (4, 9000, 64, 4, 128, "f32"), (4, 4200, 4, 4, 256, "bf16"), (16, 4100, 2, 2, 128, "f16"),
+    (8, 8300, 8, 2, 64, "f32"), (2, 9000, 34, 2, 256, "f32"),
+])
+def test_blocks_of_eight_waves(ctx, n, most, heads, kv, hd, t):
+    """Enough positions for every resident block to take eight tiles and more."""
+    g = gen(n + hd)
+    cache = Cache(g, n, kv, most, hd)
+    for lens in (lengths(n, most, 1), [most] * n, [most] + [3] * (n - 1)):
+        q = randn(g, n, heads * hd).to(DT[t])
+        out = run(ctx, cache, q, lens, range(n), heads, t, most)
+        ctx.synchronize()
+        ref, tol = kv4_64(cache, q, lens, range(n), heads, 0.09, t)
+        e = worst(out, ref, tol)
+        print(f"kv4 {n} of up to {most}, {heads}/{kv} x {hd} {t}: error / bound {e:.3f}")
+        assert e <= 1.0
+
+
 @pytest.mark.parametrize("bad", [0, 40, 63, 64, 99])
 @pytest.mark.parametrize("what", ["long", "negative", "slot", "negative slot"])
 def test_out_of_range_anywhere(ctx, bad, what):
