@@ -62,14 +62,12 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8])
     }
 }
 
-// x = hi + lo in f16
+// x = hi + lo in f16, both rounded to nearest: off by 2^-24 of x at most where lo is a normal number
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo)
 {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    hi = __builtin_bit_cast(uint32_t, h);
+    hi = pack2<_Float16>(a, b);
     const f16x2_t hv = __builtin_bit_cast(f16x2_t, hi);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hv.x), b - static_cast<float>(hv.y));
-    lo = __builtin_bit_cast(uint32_t, l);
+    lo = pack2<_Float16>(a - static_cast<float>(hv.x), b - static_cast<float>(hv.y));
 }
 
 // maximum / sum of the values of lanes l and l ^ 32
