@@ -29,14 +29,13 @@
 //     by k_prompt_planes, at a power of two for 32 keys, Q here (one for a row), P here at
 //     2^15 and the V tile's power against the smallest so far.
 //     One accumulator takes the three: no cancellation sets them apart.
-//     Bound: large calls by the matrix cores at the clock that the power limit leaves
-//     (64 query heads of 128 on 4, 8192 tokens, bf16: 1.10 ms, 1.0 PF/s of causal products;
-//     without its softmax 0.98 ms; a large matrix product reaches 1.2 PF/s), small ones by
-//     launch, tile search and first loads (~6 us) and one wave a SIMD.  f32, 32 heads on 4:
-//     4096 tokens 424 us, 512 tokens 23 us after 4 us of k_prompt_planes; on the fp32 MFMA
-//     45 us at 512.
-//   k_prompt_planes the f16 planes of f32 K and V: one read, one write (64 MB at 5 TB/s; 3 to
-//     4 us for the few blocks of a short prompt).
+//     Bound: large calls by matrix cores and VALU at the clock that the power limit leaves
+//     (64 query heads of 128 on 4, 8192 tokens, bf16: 1.02 ms, 1.08 PF/s of causal products; a
+//     large matrix product reaches 1.2), small ones by launch, tile search and first loads
+//     (~6 us) and by one wave a SIMD.  f32, 32 heads on 4: 4096 tokens 400 us, 512 tokens 22 us
+//     after 4 us of k_prompt_planes; on the fp32 MFMA 45 us at 512.
+//   k_prompt_planes the f16 planes of f32 K and V: one read, one write (34 MB of 4096 tokens
+//     in 10 us; 3 to 5 us for the few blocks of a short prompt).
 //   k_prompt_join   where the keys were split: the parts of each row rescaled to
 //     their common maximum and normalised.
 #include <algorithm>
@@ -667,14 +666,15 @@ void k_prompt_join(PromptAttn p)
 // Which form, by the blocks that a call gives and the key tiles of its longest sequence (8 query heads a KV
 // head, 4 KV heads, head_dim 128, bf16; us of the kernel, and of the join where there is one):
 //   2 x 2 waves (64 rows, two key groups: one block a CU, half the chain of tiles) while 64-row blocks leave
-//     CUs idle: 512 tokens 11.9 against 16.0 (4 x 1) and 15.1 (4 x 2);
-//   4 x 2 (128 rows) up to two such blocks a CU: 1024 tokens 24.4 / 27.0 / 26.4, 2048 53.8 / 57.5 / 77, unless
-//     there are few tiles to share out;
-//   4 x 1 beyond (two blocks a CU, nothing to merge): 4096 tokens 165 / 175 / 255, 64 sequences of 64 24 / 39 / 50.
+//     CUs idle: 512 tokens 11.2 against 15.0 (4 x 2) and 15.1 (4 x 1);
+//   4 x 2 (128 rows) up to two such blocks a CU: 1024 tokens 23.3 / 24.8 (4 x 1) / 25.2 (2 x 2), 2048 50.6 / 53.0 /
+//     71.8, unless there are few tiles to share out;
+//   4 x 1 beyond (two blocks a CU, nothing to merge): 4096 tokens 154 / 161 (4 x 2) / 234 (2 x 2), 64 sequences of
+//     64 23 / 39 / 49.
 // Keys are split over blocks (each part eight tiles or more) until every CU has one: 64 tokens behind 8000 take
-// 101 in one part of 2 x 2 and 21 + 4 in eight; over long parts 4 x 2 is ahead again (256 tokens behind 4000:
-// 30 + 5 in four parts against 36 + 4 in two of 2 x 2).  f32 (tiles of 32) by the same rule: 512 tokens 22.9
-// against 28.2 (4 x 2), 23.7 + 4.3 (4 x 1 in two parts); 1024 49.5 against 61 + 8 (2 x 2), 51 + 8 (4 x 1).
+// 89 in one part of 2 x 2 and 19 + 4 in eight; over long parts 4 x 2 is ahead again (256 tokens behind 4000:
+// 28.5 + 6.8 in four parts against 33.6 + 6.9 in two of 2 x 2).  f32 (tiles of 32) by the same rule: 512 tokens 22.7
+// against 27.8 (4 x 2), 24.3 + 4.5 (4 x 1 in two parts); 1024 48.8 / 59.5 (4 x 1); 2048 112 / 130 / 156 (2 x 2).
 void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k)
 {
     constexpr uint64_t CUS = 256;
