@@ -27,7 +27,7 @@
 //     of the rounded ones, in fp32).  f32: every operand as two f16 (hi + lo, 22 bits) and
 //     three products for one, 16 / 3 times the rate of the fp32 MFMA.  K and V are split
 //     by k_prompt_planes, at a power of two for 32 keys, Q here (one for a row), P here at
-//     2^15 and the V tile's power against the smallest so far.
+//     2^14 and the V tile's power against the smallest so far.
 //     One accumulator takes the three: no cancellation sets them apart.
 //     Bound: large calls by matrix cores and VALU at the clock that the power limit leaves
 //     (64 query heads of 128 on 4, 8192 tokens, bf16: 1.02 ms, 1.08 PF/s of causal products; a
@@ -388,7 +388,7 @@ void k_attn_prompt(PromptAttn p)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
     float mx = -INFINITY, sum = 0.f;                            // mx in powers of two
-    int vpower = NO_POWER;                                      // f32: acc holds the sum times 2^(15 + vpower)
+    int vpower = NO_POWER;                                      // f32: acc holds the sum times 2^(PLIFT + vpower)
     const int2* powers = S::F32 ? p.powers + static_cast<size_t>(kvh) * p.plane_tiles + seq.ktile : nullptr;
 
     // K operands requested ahead, and whether those of V are, as far as registers go
@@ -396,9 +396,10 @@ void k_attn_prompt(PromptAttn p)
     constexpr bool VAHEAD = !S::F32 || HD < 128;
     // The sums are rescaled when a row's maximum has grown by more than 2^SLACK, not whenever it has: with 32 rows a
     // wave one of them has a new maximum in every other tile.  Weights may then be up to 2^SLACK, which 16-bit types
-    // hold as well as 1 (f32: no slack, its f16 halves have no room).  f16: weights 2^LIFT times as large, sum and acc
-    // with them, or those under 2^-14 would be subnormal and lose bits (thousands of them may make up the sum).
-    constexpr float SLACK = S::F32 ? 0.f : 8.f, LIFT = __is_same(T, _Float16) ? 7.f : 0.f;
+    // hold as well as 1, and f32 at 2^PLIFT as f16 halves.  f16: weights 2^LIFT times as large, sum and acc with them,
+    // or those under 2^-14 would be subnormal and lose bits (thousands of them may make up the sum).
+    constexpr float SLACK = S::F32 ? 1.f : 8.f, LIFT = __is_same(T, _Float16) ? 7.f : 0.f;
+    constexpr int PLIFT = 14;
     auto tile_step = [&](int32_t t, int b, int2 pw) {
         const uint8_t* kl = mine + b * S::BUF;
         const uint8_t* vl = kl + S::PLANES * S::TILE;
@@ -491,7 +492,7 @@ void k_attn_prompt(PromptAttn p)
             mx = mn;
         }
         const float mc = (mx > -INFINITY ? mx : 0.f) - LIFT;    // (no key yet: every weight 0)
-        const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, 15 + vpower - pw.y) : 1.f;
+        const float pf = S::F32 ? __builtin_amdgcn_ldexpf(1.f, PLIFT + vpower - pw.y) : 1.f;
         // ---- weights of 16 keys, and O^T += V^T P^T of the 16 before ----
         uint4 pb[2], pl[2];
         auto weights = [&](int ks) {
@@ -580,7 +581,7 @@ void k_attn_prompt(PromptAttn p)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], -15 - vpower);
+            for (int i = 0; i < 16; ++i) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], -PLIFT - vpower);
     }
 
     // ---- the second key group's part joins the first's, lane by lane ---------------
