@@ -673,8 +673,9 @@ void k_prompt_join(PromptAttn p)
 //   4 x 1 beyond (two blocks a CU, nothing to merge): 4096 tokens 154 / 161 (4 x 2) / 234 (2 x 2), 64 sequences of
 //     64 23 / 39 / 49.
 // Keys are split over blocks (each part eight tiles or more) until every CU has one: 64 tokens behind 8000 take
-// 89 in one part of 2 x 2 and 19 + 4 in eight; over long parts 4 x 2 is ahead again (256 tokens behind 4000:
-// 28.5 + 6.8 in four parts against 33.6 + 6.9 in two of 2 x 2).  f32 (tiles of 32) by the same rule: 512 tokens 22.7
+// 89 in one part of 2 x 2 and 19 + 4 in eight; over long parts 4 x 2 is ahead again, in eight or fewer (256
+// tokens behind 4000: 28.5 + 6.8 in four against 33.6 + 6.9 in two of 2 x 2; 128 behind 16000 43 against 55, but 64
+// behind 16000 41 in sixteen against 30 in eight of 2 x 2).  f32 (tiles of 32) by the same rule: 512 tokens 22.7
 // against 27.8 (4 x 2), 24.3 + 4.5 (4 x 1 in two parts); 1024 48.8 / 59.5 (4 x 1); 2048 112 / 130 / 156 (2 x 2).
 void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k)
 {
@@ -689,7 +690,7 @@ void prompt_plan(PromptAttn& a, uint32_t head_dim, uint32_t type, uint32_t max_k
             1, std::min<uint64_t>({CUS / std::max<uint64_t>(blocks, 1), JOIN_MAX, keys / 8})));
     };
     // (LDS and registers of a CU: head_dim 256 has room for one group of four waves, or in 16 bits two of two)
-    if (!(f32 && wide) && b64 <= CUS && (wide || keys <= 24 * parts(b64))) {
+    if (!(f32 && wide) && b64 <= CUS && (wide || keys <= 24 * parts(b64) || parts(b64) >= 8)) {
         a.row_waves = 2;
         a.key_groups = 2;
         a.splits = parts(b64);
